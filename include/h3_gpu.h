@@ -106,6 +106,13 @@ int h3_gpu_tensor_read_bytes(const h3_gpu_tensor *tensor, void *bytes,
                              size_t byte_count);
 int h3_gpu_tensor_write_bytes(h3_gpu_tensor *tensor, const void *bytes,
                               size_t byte_count);
+/* Non-owning tensor over device memory of the caller's (for interop; no
+ * counterpart in the reference). The memory must outlive it, and work that
+ * other streams do on it must be over before this context's calls use it (and
+ * the other way round: h3_gpu_submit). gpu may be NULL for a tensor that only
+ * the qw_gpu_*_check functions look at. Free with h3_gpu_tensor_free. */
+h3_gpu_tensor *h3_gpu_tensor_wrap(h3_gpu *gpu, void *device_ptr,
+                                  h3_gpu_dtype dtype, size_t elements);
 /* Device address of the tensor's first element (for interop). */
 void *h3_gpu_tensor_device_ptr(const h3_gpu_tensor *tensor);
 

@@ -290,6 +290,134 @@ int qw_gpu_copy_rows(h3_gpu *gpu, h3_gpu_tensor *dst, size_t dst_offset,
                      size_t src_offset, uint32_t src_stride, uint32_t rows,
                      uint32_t row_elems);
 
+/* ---- text operators (no counterpart in the reference) -------------------
+ * What a text model's layers (a prompt's encoder or writer) run beside the
+ * image model: rotary positions, attention over a paged cache and linears on
+ * 4-bit weights. All calls enqueue on the context's stream; tensors may belong
+ * to any context of its device. The kernels are in qwen_text_kernels.hsaco,
+ * beside the code object of h3_gpu_create, loaded by the first call. The
+ * _check functions say what the calls would refuse, without a device. */
+
+/* A paged cache of grouped K/V heads and the sequences of one batch in it.
+ * Token t of sequence s lies in page table[s * table_ld + t / page_size], slot
+ * t % page_size; an entry of `pages` or more is no page: its tokens are not
+ * stored and not seen. lengths[s]: the sequence's tokens, the new ones
+ * included (at most table_ld * page_size count). Sequence s's new tokens are
+ * rows starts[s] .. starts[s + 1] - 1 of the batch, in order, the last of them
+ * its last token; starts is ascending. Rows before starts[0] and from
+ * starts[sequences] on belong to no sequence and are left as they are in every
+ * output. page_size is a power of two from 8 to 4096. Sequences may share
+ * pages that they only read; a page that a call writes belongs to one. */
+typedef struct {
+    h3_gpu_tensor *k, *v; /* bf16 [pages, page_size, kv_heads, head_dim] */
+    const h3_gpu_tensor *table;   /* u32 [sequences, table_ld] */
+    const h3_gpu_tensor *lengths; /* u32 [sequences] */
+    const h3_gpu_tensor *starts;  /* u32 [sequences + 1] */
+    uint32_t pages, page_size, table_ld, sequences, kv_heads;
+} qw_paged_cache;
+
+enum { QW_ROTARY_INTERLEAVED = 0, QW_ROTARY_HALF = 1 };
+/* Rotary positions of q and k (bf16 rows of heads x head_dim at strides of
+ * their own, for example columns of one q|k|v projection). Of each head the
+ * first rotary_dim elements turn: pairs (2 i, 2 i + 1) when interleaved, (i, i
+ * + rotary_dim / 2) for halves, pair i by positions[row] * turns[i]
+ * (qw_rope_turns) and times attention_factor; the rest passes. norm_q and
+ * norm_k, where given: the per-head RMS norm (all of head_dim, epsilon eps)
+ * ahead of the rotation. fp32 throughout, one rounding at the store.
+ *
+ * Without a cache k goes to k_out. With one, k (turned) and v (as it is) go to
+ * their tokens' places in the cache, and positions may be NULL: a token's
+ * place in its sequence. A sequence shorter than its new tokens has none of
+ * its first ones: their rows are left as they are.
+ * q_out may be q (the same rows, in place) and k_out k; otherwise outputs and
+ * inputs do not overlap. heads or kv_heads may be 0 (without a cache): then
+ * nothing is done for q or k. head_dim 64, 128 or 256; rotary_dim even, up to
+ * head_dim. Rows are 16-byte aligned. */
+typedef struct {
+    h3_gpu_tensor *q_out;
+    size_t q_out_offset;
+    uint32_t ldq_out;
+    h3_gpu_tensor *k_out;
+    size_t k_out_offset;
+    uint32_t ldk_out;
+    const h3_gpu_tensor *q;
+    size_t q_offset;
+    uint32_t ldq;
+    const h3_gpu_tensor *k;
+    size_t k_offset;
+    uint32_t ldk;
+    const h3_gpu_tensor *v; /* with a cache */
+    size_t v_offset;
+    uint32_t ldv;
+    const h3_gpu_tensor *norm_q, *norm_k; /* bf16 [head_dim], or NULL */
+    const h3_gpu_tensor *positions;       /* u32 [rows] */
+    const h3_gpu_tensor *turns;           /* u32 [rotary_dim / 2][2] */
+    const qw_paged_cache *cache;          /* or NULL */
+    uint32_t rows, heads, kv_heads, head_dim, rotary_dim;
+    int layout;             /* QW_ROTARY_* */
+    float attention_factor; /* positive; 1 for none */
+    float eps;
+} qw_rotary_desc;
+int qw_gpu_rotary_bf16(h3_gpu *gpu, const qw_rotary_desc *desc);
+int qw_gpu_rotary_check(const qw_rotary_desc *desc, char *error, size_t size);
+
+/* Causal attention of the new tokens of every sequence over all that the cache
+ * holds of it (the new ones' K/V included: qw_gpu_rotary_bf16 puts them there
+ * first): q and out bf16 [rows, heads, 128] at row strides ldq and ldo, query
+ * heads [g n, g n + n) on K/V head g, n = heads / kv_heads, any whole number.
+ * The token at place p sees the tokens (p - window, p] (window 0: [0, p]) whose
+ * page exists; what it does not see does not touch its result, whatever the
+ * cache holds there. A token that sees none gets zeros. Softmax in fp32, the
+ * probabilities rounded to bf16 for their product with V. max_new and
+ * max_length (0: not known): the most new tokens of a sequence and the longest
+ * length; hints that the launch is planned by, the result is right for any. A
+ * row's last bits may depend on them, and for one call's inputs are the same
+ * each time. */
+typedef struct {
+    h3_gpu_tensor *out;
+    size_t out_offset;
+    uint32_t ldo;
+    const h3_gpu_tensor *q;
+    size_t q_offset;
+    uint32_t ldq;
+    const qw_paged_cache *cache;
+    uint32_t rows, heads, head_dim, window, max_new, max_length;
+    float scale;
+} qw_paged_attention_desc;
+int qw_gpu_paged_attention_bf16(h3_gpu *gpu, const qw_paged_attention_desc *desc);
+int qw_gpu_paged_attention_check(const qw_paged_attention_desc *desc, char *error, size_t size);
+
+/* Y = X W^T (+ bias) on 4-bit weights: W[c][k] = (q - z) s with q the 4 bits of
+ * input k of column c (the low half of byte k / 2 for even k), s = scales[c][k /
+ * group] and z = zeros[c][k / group], 8 without zeros. Rows of in and out at
+ * strides lda and ldc. fp32 sums, one rounding. group 32, 64 or 128; k a
+ * multiple of it; cols of 8. The output overlaps no operand. */
+typedef struct {
+    h3_gpu_tensor *out;
+    size_t out_offset;
+    uint32_t ldc;
+    const h3_gpu_tensor *in;
+    size_t in_offset;
+    uint32_t lda;
+    const h3_gpu_tensor *weight; /* i8 [cols, k / 2] */
+    const h3_gpu_tensor *scales; /* bf16 [cols, k / group] */
+    const h3_gpu_tensor *zeros;  /* bf16 [cols, k / group], or NULL */
+    const h3_gpu_tensor *bias;   /* bf16 [cols], or NULL */
+    uint32_t rows, k, cols, group;
+} qw_linear_int4_desc;
+int qw_gpu_linear_int4(h3_gpu *gpu, const qw_linear_int4_desc *desc);
+int qw_gpu_linear_int4_check(const qw_linear_int4_desc *desc, char *error, size_t size);
+/* Such a weight from a bf16 one [rows, cols]. Without zeros s = bf16(max |w| /
+ * 7) and q = rint(w / s) + 8, 1 to 15; with them s = bf16((max - min) / 15) over
+ * the group and 0, z = rint(-min / s), a whole number, and q = rint(w / s) + z. */
+int qw_gpu_quantize_weight_int4(h3_gpu *gpu, h3_gpu_tensor *output, h3_gpu_tensor *scales,
+                                h3_gpu_tensor *zeros, const h3_gpu_tensor *input, uint32_t rows,
+                                uint32_t cols, uint32_t group);
+/* bf16((q - z) s) [rows, cols]. */
+int qw_gpu_dequant_int4_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *weight,
+                             const h3_gpu_tensor *scales, const h3_gpu_tensor *zeros,
+                             uint32_t rows, uint32_t cols, uint32_t group);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,6 +68,34 @@ int qw_rope_build(const int *axis_dim, int axes, qw_rope_tables *tables);
 void qw_rope_free(qw_rope_tables *tables);
 int qw_rope_row(int coordinate);
 
+/* Rotary frequencies of a text model, for qw_gpu_rotary_bf16. No counterpart
+ * in the reference, whose tables are the image model's. Pair i of n / 2 (n =
+ * rotary_dim) turns by f_i = base^(-2 i / n) radians a position, stretched for
+ * contexts past the original length L by
+ *   LINEAR    f / factor
+ *   NTK       base * factor^(n / (n - 2)) in place of base
+ *   BY_PARTS  f (k + (1 - k) / factor), k = clamp((L f / 2 pi - low) / (high -
+ *             low)): pairs of more than `high` turns over L stay, of fewer
+ *             than `low` are divided
+ *   YARN      the same with k by the pair's index: 1 up to the pair of `high`
+ *             turns over L (rounded down), 0 from that of `low` turns (rounded
+ *             up) on, linear between; attention factor 0.1 ln(factor) + 1
+ * rotary_dim is even, 2 to 256; base > 1; factor >= 1; original_length > 0 and
+ * 0 < low < high where they are used. */
+enum { QW_ROPE_PLAIN = 0, QW_ROPE_LINEAR = 1, QW_ROPE_NTK = 2, QW_ROPE_BY_PARTS = 3, QW_ROPE_YARN = 4 };
+typedef struct {
+    uint32_t rotary_dim;
+    int scaling; /* QW_ROPE_* */
+    double base, factor, original_length, low, high;
+} qw_rope_config;
+/* turns[i][0], [1]: the high and low half of f_i / 2 pi modulo 1 as a 64-bit
+ * fraction (rounded to nearest; up to the 53 bits of a double below its first
+ * one bit), so that position * turns is exact modulo a turn. attention_factor
+ * (NULL: not wanted): what the rotated part is multiplied by, 1 but for YARN.
+ * 0 and a message for a config outside the ranges above. */
+int qw_rope_turns(const qw_rope_config *config, uint32_t *turns, float *attention_factor,
+                  char *error, size_t error_size);
+
 typedef struct {
     uint64_t state;
     uint64_t increment;

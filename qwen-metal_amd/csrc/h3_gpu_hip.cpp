@@ -13,6 +13,7 @@
 #include <string.h>
 #include <time.h>
 
+#include <new>
 #include <string>
 
 #include "../../include/h3_gpu.h"
@@ -68,6 +69,7 @@ static const char *k_names[K_COUNT] = {
 enum { QW_INT8_AUTO = 0, QW_INT8_WIDEN = 1, QW_INT8_W8 = 2 };
 
 #define QW_SPAN_MAX 4096
+enum { T_COUNT = 20 }; /* kernels of the text operators (h3_gpu_text.inc) */
 
 struct h3_gpu {
     int device;
@@ -105,6 +107,10 @@ struct h3_gpu {
     /* this device's copy of the static workspace (qw_static_scratch.hip):
      * partials, then QW_STATIC_FLAGS counters */
     unsigned char *static_scratch;
+    /* the text operators' code object, loaded with the first of them */
+    char text_path[1024];
+    hipModule_t text_module;
+    hipFunction_t text_fn[T_COUNT];
 };
 
 struct h3_gpu_tensor {
@@ -188,6 +194,12 @@ extern "C" h3_gpu *h3_gpu_create(const char *code_object_path, char *error,
                "/qwen_kernels.hsaco";
     }
     h3_gpu *g = new h3_gpu();
+    {
+        const size_t slash = path.rfind('/');
+        snprintf(g->text_path, sizeof(g->text_path), "%s/qwen_text_kernels.hsaco",
+                 slash == std::string::npos ? "." : path.substr(0, slash).c_str());
+    }
+    g->text_module = NULL;
     memset(g->error, 0, sizeof(g->error));
     memset(&g->stats, 0, sizeof(g->stats));
     g->device = device;
@@ -302,6 +314,7 @@ extern "C" void h3_gpu_free(h3_gpu *g) {
     hipEventDestroy(g->chain0);
     hipEventDestroy(g->chain1);
     hipStreamDestroy(g->stream);
+    if (g->text_module) hipModuleUnload(g->text_module);
     hipModuleUnload(g->module);
     delete g;
 }
@@ -519,6 +532,25 @@ extern "C" h3_gpu_tensor *h3_gpu_tensor_view(const h3_gpu_tensor *base, size_t o
     }
     return new h3_gpu_tensor{base->gpu, base->ptr + offset * dtype_size(base->dtype), elements,
                              base->dtype, 0};
+}
+
+extern "C" h3_gpu_tensor *h3_gpu_tensor_wrap(h3_gpu *g, void *device_ptr, h3_gpu_dtype dtype,
+                                             size_t elements) {
+    if (!device_ptr && elements) {
+        fail(g, "wrap: no address");
+        return NULL;
+    }
+    if (dtype != H3_GPU_F32 && dtype != H3_GPU_BF16 && dtype != H3_GPU_I8 && dtype != H3_GPU_U32) {
+        fail(g, "wrap: unknown dtype %d", (int)dtype);
+        return NULL;
+    }
+    if (elements > SIZE_MAX / 4 || (uintptr_t)device_ptr % dtype_size(dtype)) {
+        fail(g, "wrap: too many elements, or an address off the type's alignment");
+        return NULL;
+    }
+    h3_gpu_tensor *t = new (std::nothrow) h3_gpu_tensor{g, (unsigned char *)device_ptr, elements, dtype, 0};
+    if (!t) fail(g, "wrap: out of host memory");
+    return t;
 }
 
 extern "C" void h3_gpu_tensor_free(h3_gpu_tensor *t) {
@@ -1932,3 +1964,5 @@ extern "C" int h3_gpu_gqa_causal_bf16(h3_gpu *g, h3_gpu_tensor *out, const h3_gp
     if (kvh != qh) return fail(g, "gqa_causal: grouped K/V heads not supported");
     return sdpa_contig(g, out, q, k, v, NULL, seq, seq, qh, head_dim, scale, seq, 1);
 }
+
+#include "h3_gpu_text.inc"

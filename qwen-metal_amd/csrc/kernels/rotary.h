@@ -1,0 +1,154 @@
+/* Rotary positions of q and k, with the per-head RMS norm ahead of them where
+ * there is one, and k and v going into a paged cache.
+ *
+ * Pair i of a head turns by position * f_i, f_i in turns as a 64-bit
+ * fraction: the product modulo one turn is exact in integer arithmetic (its
+ * top 32 bits are pos * high + mulhi(pos, low)), however far the position,
+ * where a product in fp32 is off by a radian at a position of 2^24. What is
+ * left of the turn is brought to an eighth either way and goes into the
+ * series of sine and cosine. Norm and rotation stay in fp32 and are rounded
+ * once, at the store.
+ *
+ * Bound by HBM for many rows, by latency for few. A workgroup has one row and
+ * 256 / (head_dim / 8) of its heads, a lane 16 bytes: the row's sines are made
+ * once per workgroup and shared through LDS (made by every lane for itself
+ * they cost 8 pairs for each 16 bytes, more than the bytes' time). */
+#pragma once
+#include "common.h"
+#include "paged_cache.h"
+
+/* (cos, sin) of a 32-bit fraction of a turn: a quarter turn's multiple off the
+ * top, the rest x in [-pi/4, pi/4] by the Taylor series (remainders x^11/11! <
+ * 2e-9 and x^10/10! < 3e-8). */
+__device__ __forceinline__ qw_f2 rotary_cos_sin(uint32_t turn) {
+    const uint32_t quarter = (turn + 0x20000000u) >> 30;
+    const float x = (float)(int32_t)(turn - (quarter << 30)) * 1.46291807926715968e-9f; /* 2 pi / 2^32 */
+    const float y = x * x;
+    const float s = x * __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), 1.0f);
+    const float c = __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, 1.0f / 40320, -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
+    const float a = quarter & 1 ? s : c, b = quarter & 1 ? c : s;
+    return qw_f2{quarter == 1 || quarter == 2 ? -a : a, quarter >= 2 ? -b : b};
+}
+
+/* How many of starts[1..n] are at or below `row`: the sequence of a row, all
+ * 64 lanes together. */
+__device__ __forceinline__ uint32_t rotary_sequence(const qw_cache_args &c, uint32_t row) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t n = 0;
+    for (uint32_t s = 0; s < c.sequences; s += 64) {
+        const bool below = s + lane < c.sequences && c.starts[s + lane + 1] <= row;
+        n += __popcll(__builtin_amdgcn_ballot_w64(below));
+    }
+    return n;
+}
+
+template <int D>
+__device__ __forceinline__ void rotary_impl(const qw_rotary_args &a) {
+    constexpr uint32_t LPH = D / 8; /* lanes per head */
+    __shared__ qw_f2 turned[D / 2];
+    const uint32_t tid = threadIdx.x, row = blockIdx.x;
+    const uint32_t head = blockIdx.y * (256 / LPH) + tid / LPH, c8 = tid % LPH * 8;
+    const uint32_t all = a.heads + a.kv_heads * (a.cached ? 2 : 1);
+    const bool live = head < all;
+    const bool is_q = head < a.heads, is_k = !is_q && head < a.heads + a.kv_heads;
+    const uint32_t kvh = is_q ? 0 : is_k ? head - a.heads : head - a.heads - a.kv_heads;
+    const u16 *src = is_q   ? a.q + (size_t)row * a.ldq + head * D
+                     : is_k ? a.k + (size_t)row * a.ldk + kvh * D
+                            : a.v + (size_t)row * a.ldv + kvh * D;
+    /* the row's own values, and those that they are paired with */
+    const uint32_t hn = a.rotary_dim / 2;
+    const bool turns = live && (is_q || is_k), pairs = turns && a.half && c8 < a.rotary_dim;
+    u32x4 own = {0, 0, 0, 0}, other = {0, 0, 0, 0};
+    if (live) own = *(const u32x4 *)(src + c8);
+    /* element e pairs with e + hn below hn and e - hn from there on */
+    const bool whole = hn % 8 == 0; /* a lane's partners lie in one chunk */
+    if (pairs && whole) other = *(const u32x4 *)(src + (c8 < hn ? c8 + hn : c8 - hn));
+    if (pairs && !whole) {
+        u16 t[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t e = c8 + i;
+            t[i] = e < hn ? src[e + hn] : e < a.rotary_dim ? src[e - hn] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) other[i] = t[2 * i] | (uint32_t)t[2 * i + 1] << 16;
+    }
+
+    uint32_t pos = 0;
+    uint64_t at = ~0ull; /* of the cache */
+    if (a.cached) {
+        const uint32_t s = rotary_sequence(a.cache, row);
+        if (s == a.cache.sequences) return; /* behind the last sequence */
+        const qw_span sp = qw_cache_span(a.cache, s, a.rows);
+        if (row < sp.begin || row - sp.begin >= sp.rows) return;
+        const int64_t place = qw_cache_place(sp, row - sp.begin);
+        if (place < 0) return; /* a token that its sequence does not have */
+        pos = (uint32_t)place;
+        const uint32_t page = a.cache.table[qw_cache_entry(a.cache, s, pos)];
+        if (page < a.cache.pages) at = qw_cache_at(a.cache, page, pos, kvh, D);
+    }
+    if (a.positions) pos = a.positions[row];
+    if (tid < hn) {
+        const u32x2 t = *(const u32x2 *)(a.turns + 2 * tid);
+        const qw_f2 cs = rotary_cos_sin(pos * t[0] + __umulhi(pos, t[1]));
+        turned[tid] = qw_f2{cs[0] * a.factor, cs[1] * a.factor};
+    }
+    __syncthreads();
+    if (!live) return;
+
+    if (turns) {
+        float x[8], y[8];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[2 * i] = lo_bf(own[i]), x[2 * i + 1] = hi_bf(own[i]);
+            y[2 * i] = lo_bf(other[i]), y[2 * i + 1] = hi_bf(other[i]);
+        }
+        const u16 *w = is_q ? a.norm_q : a.norm_k;
+        if (w) {
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) s = __builtin_fmaf(x[i], x[i], s);
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+            const float inv = __builtin_amdgcn_rsqf(__builtin_fmaf(s, 1.0f / D, a.eps));
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                const uint32_t e = c8 + i;
+                x[i] *= inv * bf2f(w[e]);
+                if (pairs && e < a.rotary_dim) y[i] *= inv * bf2f(w[e < hn ? e + hn : e - hn]);
+            }
+        }
+        float z[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) z[i] = x[i];
+        if (a.half) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                const uint32_t e = c8 + i;
+                if (e >= a.rotary_dim) continue;
+                const qw_f2 t = turned[e < hn ? e : e - hn];
+                z[i] = e < hn ? x[i] * t[0] - y[i] * t[1] : y[i] * t[1] + x[i] * t[0];
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i += 2) {
+                if (c8 + i >= a.rotary_dim) continue;
+                const qw_f2 t = turned[(c8 + i) / 2];
+                z[i] = x[i] * t[0] - x[i + 1] * t[1];
+                z[i + 1] = x[i] * t[1] + x[i + 1] * t[0];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) own[i] = pack_bf(z[2 * i], z[2 * i + 1]);
+    }
+    if (is_q) {
+        *(u32x4 *)(a.q_out + (size_t)row * a.ldq_out + head * D + c8) = own;
+    } else if (!a.cached) {
+        *(u32x4 *)(a.k_out + (size_t)row * a.ldk_out + kvh * D + c8) = own;
+    } else if (at != ~0ull) {
+        *(u32x4 *)((is_k ? a.cache.k : a.cache.v) + at + c8) = own;
+    }
+}
+QW_KERNEL void __launch_bounds__(256) qw_rotary_d64(qw_rotary_args a) { rotary_impl<64>(a); }
+QW_KERNEL void __launch_bounds__(256) qw_rotary_d128(qw_rotary_args a) { rotary_impl<128>(a); }
+QW_KERNEL void __launch_bounds__(256) qw_rotary_d256(qw_rotary_args a) { rotary_impl<256>(a); }

@@ -5,6 +5,7 @@
 #include "../../include/qwen_host.h"
 
 #include <math.h>
+#include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
 
@@ -110,6 +111,55 @@ void qw_rope_free(qw_rope_tables *t) {
     free(t->cos);
     free(t->sin);
     t->cos = t->sin = NULL;
+}
+
+static int rope_bad(char *error, size_t size, const char *what) {
+    if (error && size) snprintf(error, size, "rope turns: %s", what);
+    return 0;
+}
+
+int qw_rope_turns(const qw_rope_config *c, uint32_t *turns, float *attention_factor, char *error,
+                  size_t error_size) {
+    const double two_pi = 6.283185307179586476925286766559;
+    if (!c || !turns) return rope_bad(error, error_size, "no config or no table");
+    const uint32_t n = c->rotary_dim;
+    if (n < 2 || n % 2 || n > 256) return rope_bad(error, error_size, "rotary_dim is not even, 2 to 256");
+    if (!(c->base > 1.0) || !isfinite(c->base)) return rope_bad(error, error_size, "base is not above 1");
+    const int how = c->scaling, parts = how == QW_ROPE_BY_PARTS || how == QW_ROPE_YARN;
+    if (how < QW_ROPE_PLAIN || how > QW_ROPE_YARN) return rope_bad(error, error_size, "unknown scaling");
+    if (how != QW_ROPE_PLAIN && (!(c->factor >= 1.0) || !isfinite(c->factor)))
+        return rope_bad(error, error_size, "factor is not 1 or more");
+    if (how == QW_ROPE_NTK && n < 4) return rope_bad(error, error_size, "NTK needs two pairs");
+    if (parts && (!(c->original_length > 0.0) || !isfinite(c->original_length) || !(c->low > 0.0) ||
+                  !(c->high > c->low) || !isfinite(c->high)))
+        return rope_bad(error, error_size, "original_length, low or high out of range");
+    double base = c->base, first = 0.0, last = 0.0;
+    if (how == QW_ROPE_NTK) base *= pow(c->factor, n / (n - 2.0));
+    if (how == QW_ROPE_YARN) {
+        /* the pair that makes t turns over the length */
+        const double per = n / (2.0 * log(base));
+        first = fmax(floor(per * log(c->original_length / (c->high * two_pi))), 0.0);
+        last = fmin(ceil(per * log(c->original_length / (c->low * two_pi))), n - 1.0);
+    }
+    for (uint32_t i = 0; i < n / 2; i++) {
+        double f = pow(base, -2.0 * i / n), keep = 1.0;
+        if (how == QW_ROPE_LINEAR) keep = 0.0;
+        if (how == QW_ROPE_BY_PARTS)
+            keep = fmin(fmax((c->original_length * f / two_pi - c->low) / (c->high - c->low), 0.0), 1.0);
+        if (how == QW_ROPE_YARN)
+            keep = 1.0 - fmin(fmax((i - first) / fmax(last - first, 0.001), 0.0), 1.0);
+        if (keep < 1.0) f *= keep + (1.0 - keep) / c->factor;
+        double t = f / two_pi; /* below 1: base > 1 */
+        t -= floor(t);
+        /* a double in [0, 1) times 2^64; below 2^-11 some low bits are its own */
+        const double scaled = ldexp(t, 64);
+        const uint64_t u = scaled >= 18446744073709551615.0 ? UINT64_MAX : (uint64_t)rint(scaled);
+        turns[2 * i] = (uint32_t)(u >> 32);
+        turns[2 * i + 1] = (uint32_t)u;
+    }
+    if (attention_factor)
+        *attention_factor = how == QW_ROPE_YARN ? (float)(0.1 * log(c->factor) + 1.0) : 1.0f;
+    return 1;
 }
 
 uint32_t qw_rng_u32(qw_rng *r) {

@@ -80,6 +80,51 @@ class ConditioningDesc(C.Structure):
         ("rows", u32), ("hidden", u32), ("shift_variant", C.c_int)]
 
 
+ROTARY_INTERLEAVED, ROTARY_HALF = 0, 1
+ROPE_INTERLEAVED, ROPE_HALF = ROTARY_INTERLEAVED, ROTARY_HALF
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_BY_PARTS, ROPE_YARN = 0, 1, 2, 3, 4
+
+
+class RopeConfig(C.Structure):
+    """qw_rope_config (include/qwen_host.h)"""
+    _fields_ = [("rotary_dim", u32), ("scaling", C.c_int), ("base", C.c_double),
+                ("factor", C.c_double), ("original_length", C.c_double), ("low", C.c_double),
+                ("high", C.c_double)]
+
+
+class PagedCache(C.Structure):
+    """qw_paged_cache (include/qwen_gpu_ext.h)"""
+    _fields_ = [(n, vp) for n in ("k", "v", "table", "lengths", "starts")] + [
+        (n, u32) for n in ("pages", "page_size", "table_ld", "sequences", "kv_heads")]
+
+
+class RotaryDesc(C.Structure):
+    """qw_rotary_desc"""
+    _fields_ = [("q_out", vp), ("q_out_offset", sz), ("ldq_out", u32), ("k_out", vp),
+                ("k_out_offset", sz), ("ldk_out", u32), ("q", vp), ("q_offset", sz),
+                ("ldq", u32), ("k", vp), ("k_offset", sz), ("ldk", u32), ("v", vp),
+                ("v_offset", sz), ("ldv", u32), ("norm_q", vp), ("norm_k", vp),
+                ("positions", vp), ("turns", vp), ("cache", C.POINTER(PagedCache)),
+                ("rows", u32), ("heads", u32), ("kv_heads", u32), ("head_dim", u32),
+                ("rotary_dim", u32), ("layout", C.c_int), ("attention_factor", C.c_float),
+                ("eps", C.c_float)]
+
+
+class PagedAttentionDesc(C.Structure):
+    """qw_paged_attention_desc"""
+    _fields_ = [("out", vp), ("out_offset", sz), ("ldo", u32), ("q", vp), ("q_offset", sz),
+                ("ldq", u32), ("cache", C.POINTER(PagedCache)), ("rows", u32), ("heads", u32),
+                ("head_dim", u32), ("window", u32), ("max_new", u32), ("max_length", u32),
+                ("scale", C.c_float)]
+
+
+class LinearInt4Desc(C.Structure):
+    """qw_linear_int4_desc"""
+    _fields_ = [("out", vp), ("out_offset", sz), ("ldc", u32), ("in_", vp), ("in_offset", sz),
+                ("lda", u32), ("weight", vp), ("scales", vp), ("zeros", vp), ("bias", vp),
+                ("rows", u32), ("k", u32), ("cols", u32), ("group", u32)]
+
+
 # Every exported entry point with its (restype, argtypes). The CPU test
 # checks the library exports each name declared in include/*.h.
 SIGNATURES = {
@@ -93,6 +138,7 @@ SIGNATURES = {
     "h3_gpu_tensor_from_bf16": (vp, [vp, vp, sz]),
     "h3_gpu_tensor_from_u32": (vp, [vp, vp, sz]),
     "h3_gpu_tensor_view": (vp, [vp, sz, sz]),
+    "h3_gpu_tensor_wrap": (vp, [vp, vp, C.c_int, sz]),
     "h3_gpu_tensor_free": (None, [vp]),
     "h3_gpu_tensor_elements": (sz, [vp]),
     "h3_gpu_tensor_dtype": (C.c_int, [vp]),
@@ -152,6 +198,16 @@ SIGNATURES = {
     "qw_gpu_widen_int8_bf16": (C.c_int, [vp, vp, vp, sz]),
     "qw_gpu_cfg_euler_f32": (C.c_int, [vp, vp, vp, sz, vp, sz, sz, C.c_float, C.c_float]),
     "qw_gpu_copy_rows": (C.c_int, [vp, vp, sz, u32, vp, sz, u32, u32, u32]),
+    "qw_gpu_rotary_bf16": (C.c_int, [vp, C.POINTER(RotaryDesc)]),
+    "qw_gpu_rotary_check": (C.c_int, [C.POINTER(RotaryDesc), C.c_char_p, sz]),
+    "qw_gpu_paged_attention_bf16": (C.c_int, [vp, C.POINTER(PagedAttentionDesc)]),
+    "qw_gpu_paged_attention_check": (C.c_int, [C.POINTER(PagedAttentionDesc), C.c_char_p, sz]),
+    "qw_gpu_linear_int4": (C.c_int, [vp, C.POINTER(LinearInt4Desc)]),
+    "qw_gpu_linear_int4_check": (C.c_int, [C.POINTER(LinearInt4Desc), C.c_char_p, sz]),
+    "qw_gpu_quantize_weight_int4": (C.c_int, [vp, vp, vp, vp, vp, u32, u32, u32]),
+    "qw_gpu_dequant_int4_bf16": (C.c_int, [vp, vp, vp, vp, vp, u32, u32, u32]),
+    "qw_rope_turns": (C.c_int, [C.POINTER(RopeConfig), vp, C.POINTER(C.c_float), C.c_char_p,
+                                sz]),
     "qw_dit_config_reference": (None, [C.POINTER(DitConfig)]),
     "qw_dit_config_baseline": (None, [C.POINTER(DitConfig)]),
     "qw_dit_create": (vp, [vp, C.c_char_p, C.c_int, C.c_char_p, sz]),
@@ -247,6 +303,17 @@ def lib():
     return _LIB
 
 
+def rope_turns(rotary_dim, base=10000.0, scaling=ROPE_PLAIN, factor=1.0, original_length=0.0,
+               low=0.0, high=0.0):
+    """(turns u32 [rotary_dim / 2, 2], attention factor) of qw_rope_turns"""
+    config = RopeConfig(rotary_dim, scaling, base, factor, original_length, low, high)
+    turns = np.zeros((max(rotary_dim // 2, 1), 2), np.uint32)
+    size, err = C.c_float(), C.create_string_buffer(256)
+    if not lib().qw_rope_turns(C.byref(config), _p(turns), C.byref(size), err, 256):
+        raise ValueError(err.value.decode())
+    return turns, size.value
+
+
 def _p(a):
     return a.ctypes.data_as(vp)
 
@@ -304,6 +371,14 @@ class Gpu:
         fn = {F32: "h3_gpu_tensor_new_f32", BF16: "h3_gpu_tensor_new_bf16",
               I8: "h3_gpu_tensor_new_i8", U32: "h3_gpu_tensor_new_u32"}[dtype]
         h = getattr(lib(), fn)(self.h, n)
+        if not h:
+            raise RuntimeError(self.error())
+        return Tensor(self, h, n, dtype)
+
+    def wrap(self, ptr, n, dtype):
+        """A library tensor over device memory of the caller's, who keeps it
+        alive."""
+        h = lib().h3_gpu_tensor_wrap(self.h, ptr, dtype, n)
         if not h:
             raise RuntimeError(self.error())
         return Tensor(self, h, n, dtype)
