@@ -45,46 +45,216 @@ __device__ __forceinline__ u32x4 l4_transpose(u32x4 w) {
     return u32x4{(uint32_t)t[0], (uint32_t)t[1], (uint32_t)u[0], (uint32_t)u[1]};
 }
 
-/* NT: tiles of 16 rows, CT: tiles of 16 columns per workgroup, GS: group */
-template <int NT, int CT, int GS>
-__device__ __forceinline__ void linear4_impl(const qw_linear4_args &a) {
-    __shared__ float part[L4_WAVES / 2][CT * NT * 256];
-    const uint32_t lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t col0 = blockIdx.x * 16 * CT, groups = a.k / GS, steps = (a.k + 127) / 128;
+/* What a step of 128 inputs takes of a column tile: 16 bytes of weights a lane
+ * and the groups' scales and zero points (Z: there are some). Steps past the
+ * last are read as it: no branch stands between a load and its use, where the
+ * compiler would wait for every load. */
+template <int GS, bool Z>
+struct l4_step {
+    u32x4 q;
+    u16 s[128 / GS], z[128 / GS];
+};
+template <int GS, bool Z>
+__device__ __forceinline__ void l4_load(const qw_linear4_args &a, l4_step<GS, Z> &w, uint32_t col,
+                                        uint32_t st, uint32_t g) {
+    const uint32_t groups = a.k / GS, steps = (a.k + 127) / 128, k0 = min(st, steps - 1) * 128;
+    uint32_t at = k0 + 32 * g;
+    if (GS < 128) at = min(at, a.k - 32);
+    w.q = *(const u32x4 *)(a.weight + ((size_t)col * a.k + at) / 2);
+    const size_t gi = (size_t)col * groups;
+#pragma unroll
+    for (int n = 0; n < 128 / GS; n++) {
+        const size_t e = gi + min(k0 / GS + n, groups - 1);
+        w.s[n] = a.scales[e];
+        w.z[n] = Z ? a.zeros[e] : 0x4100; /* 8 */
+    }
+}
+
+/* ---- up to 16 rows that fit LDS ------------------------------------------- */
+
+/* A workgroup takes tiles of 16 columns, its 8 waves every 8th step of them.
+ * All of x lies in LDS, in the order that l4_widen gives weights, and a tile's
+ * scales and zero points (one block of memory) are copied there a tile ahead:
+ * as 2-byte loads, two of each a step at groups of 64, they took as long as
+ * the weights (12288 -> 4096, one row: 21.0 us against 10.3 with groups of 128
+ * and no zero points). Weights are loaded L4_AHEAD steps before their use,
+ * over the end of a tile into the next. Rows past the last are computed as it,
+ * and not stored; so are columns. */
+#define L4_AHEAD 4
+#define L4_LDS 65536 /* x, then two buffers of scales and zero points */
+template <int GS, bool Z>
+__device__ __forceinline__ void linear4_few(const qw_linear4_args &a) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[L4_LDS];
+    __shared__ float part[L4_WAVES][256];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t steps = (a.k + 127) / 128, tiles = (a.cols + 15) / 16, groups = a.k / GS;
     const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u,
                                                          0x3F803F80u});
-    /* columns past the last are computed as it, and not stored; so are rows */
-    uint32_t col[CT];
-    const uint8_t *w[CT];
-    const u16 *x[NT];
+    u32x4 w[L4_AHEAD];
+    auto load = [&](int u, uint32_t tile, uint32_t st) __attribute__((always_inline)) {
+        const uint32_t col = min(min(tile, tiles - 1) * 16 + i, a.cols - 1);
+        uint32_t at = min(st, steps - 1) * 128 + 32 * g;
+        if (GS < 128) at = min(at, a.k - 32);
+        w[u] = *(const u32x4 *)(a.weight + ((size_t)col * a.k + at) / 2);
+    };
+    uint32_t tile = blockIdx.x;
 #pragma unroll
-    for (int c = 0; c < CT; c++) {
-        col[c] = min(col0 + 16 * c + i, a.cols - 1);
-        w[c] = a.weight + (size_t)col[c] * (a.k / 2) + 16 * g;
+    for (int u = 0; u < L4_AHEAD; u++) load(u, tile, wave + u * L4_WAVES);
+    /* scales of a tile: `groups` of 16 columns; a column's row in LDS is 4
+     * bytes longer, so that the lanes' reads hit different banks */
+    const uint32_t srow = groups * 2 + (groups & 1 ? 2 : 4), sbytes = 16 * srow;
+    unsigned char *const sl = lds + (size_t)a.rows * steps * 256;
+    auto copy_scales = [&](uint32_t t, uint32_t buffer) __attribute__((always_inline)) {
+        for (uint32_t e = tid * 2; e < 16 * groups; e += 2 * 64 * L4_WAVES) {
+            /* two neighbours; a pair may pass from a column to the next */
+            const uint64_t at = min((uint64_t)t * 16 * groups + e, (uint64_t)a.cols * groups - 2);
+            const uint32_t s = *(const uint32_t *)(a.scales + at);
+            const uint32_t z = Z ? *(const uint32_t *)(a.zeros + at) : 0;
+            unsigned char *to = sl + buffer * sbytes * (1 + Z);
+            const uint32_t c0 = e / groups, c1 = (e + 1) / groups;
+            *(u16 *)(to + c0 * srow + (e - c0 * groups) * 2) = (u16)s;
+            *(u16 *)(to + c1 * srow + (e + 1 - c1 * groups) * 2) = (u16)(s >> 16);
+            if (Z) {
+                *(u16 *)(to + sbytes + c0 * srow + (e - c0 * groups) * 2) = (u16)z;
+                *(u16 *)(to + sbytes + c1 * srow + (e + 1 - c1 * groups) * 2) = (u16)(z >> 16);
+            }
+        }
+    };
+    copy_scales(tile, 0);
+    /* 16-byte chunk ch of a row at ch ^ (row % 16); zeros behind k */
+    for (uint32_t row = 0; row < a.rows; row++)
+        for (uint32_t ch = tid; ch < steps * 16; ch += 64 * L4_WAVES) {
+            u32x4 v = {0, 0, 0, 0};
+            if (8 * ch < a.k) v = *(const u32x4 *)(a.in + (size_t)row * a.lda + 8 * ch);
+            *(bf16x8 *)(lds + row * steps * 256 + ((ch ^ (row & 15)) << 4)) = l4_order(v);
+        }
+    __syncthreads();
+    floatx4 sum = {0, 0, 0, 0};
+    const uint32_t xrow = min(i, a.rows - 1);
+    const unsigned char *const xr = lds + xrow * steps * 256;
+    auto step = [&](int u, uint32_t st, const unsigned char *sc) __attribute__((always_inline)) {
+        const u32x4 q = GS == 128 ? w[u] : l4_transpose(w[u]);
+#pragma unroll
+        for (int n = 0; n < 128 / GS; n++) {
+            floatx4 xs = {0, 0, 0, 0}, p = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = n * GS / 32; j < (n + 1) * GS / 32; j++) {
+                const uint32_t ch = st * 16 + (GS == 128 ? 4 * g + j : 4 * j + g);
+                const bf16x8 xf = *(const bf16x8 *)(xr + ((ch ^ xrow) << 4));
+                xs = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, ones, xs, 0, 0, 0);
+                p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, l4_widen(q[j]), p, 0, 0, 0);
+            }
+            const uint32_t gi = min(st * (128 / GS) + n, groups - 1) * 2; /* past k: x is zero */
+            const float s = bf2f(*(const u16 *)(sc + gi));
+            const float z = Z ? -128.0f - bf2f(*(const u16 *)(sc + sbytes + gi)) : -136.0f;
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                sum[r] = __builtin_fmaf(s, __builtin_fmaf(z, xs[r], p[r]), sum[r]);
+        }
+    };
+    for (uint32_t buffer = 0; tile < tiles; tile += gridDim.x, buffer ^= 1) {
+        const unsigned char *const sc = sl + buffer * sbytes * (1 + Z) + i * srow;
+        for (uint32_t base = 0; base < steps; base += L4_AHEAD * L4_WAVES) {
+            const bool end = base + L4_AHEAD * L4_WAVES >= steps;
+            const uint32_t to = end ? tile + gridDim.x : tile;
+            const uint32_t from = wave + (end ? 0 : base + L4_AHEAD * L4_WAVES);
+#pragma unroll
+            for (int u = 0; u < L4_AHEAD; u++) {
+                const uint32_t st = base + u * L4_WAVES + wave;
+                if (st < steps) step(u, st, sc);
+                load(u, to, from + u * L4_WAVES);
+            }
+        }
+        if (tile + gridDim.x < tiles) copy_scales(tile + gridDim.x, buffer ^ 1);
+        /* row 4 g + r, column i: the waves' sums meet in LDS */
+        *(floatx4 *)&part[wave][lane * 4] = sum;
+        sum = floatx4{0, 0, 0, 0};
+        __syncthreads();
+        const uint32_t row = tid >> 4, c = tid & 15, col = tile * 16 + c;
+        if (tid < 256 && row < a.rows && col < a.cols) {
+            float y = 0.0f;
+#pragma unroll
+            for (int n = 0; n < L4_WAVES; n++) y += part[n][((row >> 2) * 16 + c) * 4 + (row & 3)];
+            a.out[(size_t)row * a.ldc + col] = f2bf(y + (a.bias ? bf2f(a.bias[col]) : 0.0f));
+        }
+        __syncthreads();
     }
+}
+#define L4_FEW(gs)                                                                             \
+    QW_KERNEL void __launch_bounds__(64 * L4_WAVES, 4) qw_linear4_few_g##gs(qw_linear4_args a) { \
+        linear4_few<gs, false>(a);                                                             \
+    }                                                                                          \
+    QW_KERNEL void __launch_bounds__(64 * L4_WAVES, 4) qw_linear4_few_g##gs##z(qw_linear4_args a) { \
+        linear4_few<gs, true>(a);                                                              \
+    }
+L4_FEW(32) L4_FEW(64) L4_FEW(128)
+
+/* ---- up to 64 rows ------------------------------------------------------- */
+
+/* x weighs as much as the weight: 16 columns a workgroup read it from L2
+ * 1536 times for 24576 columns (98.8 us at 60 rows). A workgroup has 128
+ * columns, 32 for each of 4 waves, and two such sets of waves on alternate
+ * slabs of 128 inputs; x's slabs pass through LDS, in the order that l4_widen
+ * gives weights, one pair of slabs ahead. Few columns are cut along K in
+ * a.pieces ranges that meet in memory (the last in adds them in order). NT:
+ * tiles of 16 rows. */
+#define L4_COLS 128
+template <int NT, int GS, bool Z>
+__device__ __forceinline__ void linear4_many(const qw_linear4_args &a) {
+    constexpr int ROWS = 16 * NT, CT = 2, SLAB = ROWS * 256; /* bytes */
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2][2 * SLAB];
+    __shared__ uint32_t arrived;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), set = wave >> 2;
+    const uint32_t piece = blockIdx.x % a.pieces, tile = blockIdx.x / a.pieces;
+    const uint32_t col0 = tile * L4_COLS + (wave & 3) * 32;
+    const uint32_t slabs = (a.k + 127) / 128;
+    const uint32_t first = (uint64_t)slabs * piece / a.pieces;
+    const uint32_t last = (uint64_t)slabs * (piece + 1) / a.pieces;
+    const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u,
+                                                         0x3F803F80u});
+    uint32_t col[CT];
 #pragma unroll
-    for (int t = 0; t < NT; t++)
-        x[t] = a.in + (size_t)min(16 * t + i, a.rows - 1) * a.lda + (GS == 128 ? 32 : 8) * g;
+    for (int c = 0; c < CT; c++) col[c] = min(col0 + 16 * c + i, a.cols - 1);
+    /* x: chunk n of a thread is 16 bytes of a row of one of the two slabs;
+     * chunk ch of a row lies at ch ^ (row % 16) */
+    u32x4 xv[NT];
+    auto load_x = [&](uint32_t slab) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const uint32_t c = n * 512 + tid, row = (c >> 4) % ROWS;
+            const uint32_t k = (slab + c / (ROWS * 16)) * 128 + (c & 15) * 8;
+            xv[n] = u32x4{0, 0, 0, 0};
+            if (k < a.k) xv[n] = *(const u32x4 *)(a.in + (size_t)min(row, a.rows - 1) * a.lda + k);
+        }
+    };
+    auto store_x = [&](uint32_t buffer) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const uint32_t c = n * 512 + tid, row = (c >> 4) % ROWS;
+            *(bf16x8 *)(lds[buffer] + c / (ROWS * 16) * SLAB + row * 256 +
+                        (((c & 15) ^ (row & 15)) << 4)) = l4_order(xv[n]);
+        }
+    };
+    l4_step<GS, Z> w[2][CT];
+    auto load_w = [&](int u, uint32_t slab) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < CT; c++) l4_load(a, w[u][c], col[c], slab, g);
+    };
     floatx4 sum[CT][NT];
 #pragma unroll
     for (int c = 0; c < CT; c++)
 #pragma unroll
         for (int t = 0; t < NT; t++) sum[c][t] = floatx4{0, 0, 0, 0};
-
-    for (uint32_t st = wave; st < steps; st += L4_WAVES) {
-        const uint32_t k0 = st * 128;
+    auto step = [&](int u, uint32_t buffer, uint32_t k0) __attribute__((always_inline)) {
+        const unsigned char *xs_ = lds[buffer] + set * SLAB;
         u32x4 q[CT];
 #pragma unroll
-        for (int c = 0; c < CT; c++) {
-            q[c] = u32x4{0, 0, 0, 0};
-            if (GS == 128 || k0 + 32 * g < a.k) q[c] = *(const u32x4 *)(w[c] + k0 / 2);
-            if (GS < 128) q[c] = l4_transpose(q[c]);
-        }
+        for (int c = 0; c < CT; c++) q[c] = GS == 128 ? w[u][c].q : l4_transpose(w[u][c].q);
 #pragma unroll
-        for (int j0 = 0; j0 < 4; j0 += GS / 32) { /* a group */
-            if (GS < 128 && k0 + 32 * j0 >= a.k) break;
-            const uint32_t gi = (k0 + 32 * j0) / GS;
+        for (int n = 0; n < 128 / GS; n++) {
+            if (GS < 128 && k0 + n * GS >= a.k) break;
             floatx4 xs[NT], p[CT][NT];
 #pragma unroll
             for (int t = 0; t < NT; t++) {
@@ -93,14 +263,14 @@ __device__ __forceinline__ void linear4_impl(const qw_linear4_args &a) {
                 for (int c = 0; c < CT; c++) p[c][t] = floatx4{0, 0, 0, 0};
             }
 #pragma unroll
-            for (int j = j0; j < j0 + GS / 32; j++) {
+            for (int j = n * GS / 32; j < (n + 1) * GS / 32; j++) {
                 bf16x8 wf[CT];
 #pragma unroll
                 for (int c = 0; c < CT; c++) wf[c] = l4_widen(q[c][j]);
+                const uint32_t ch = GS == 128 ? 4 * g + j : 4 * j + g;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const bf16x8 xf = l4_order(
-                        *(const u32x4 *)(x[t] + k0 + (GS == 128 ? 8 : 32) * j));
+                    const bf16x8 xf = *(const bf16x8 *)(xs_ + (16 * t + i) * 256 + ((ch ^ i) << 4));
                     xs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, ones, xs[t], 0, 0, 0);
 #pragma unroll
                     for (int c = 0; c < CT; c++)
@@ -109,9 +279,7 @@ __device__ __forceinline__ void linear4_impl(const qw_linear4_args &a) {
             }
 #pragma unroll
             for (int c = 0; c < CT; c++) {
-                const size_t at = (size_t)col[c] * groups + gi;
-                const float s = bf2f(a.scales[at]);
-                const float z = -128.0f - (a.zeros ? bf2f(a.zeros[at]) : 8.0f);
+                const float s = bf2f(w[u][c].s[n]), z = -128.0f - bf2f(w[u][c].z[n]);
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -120,28 +288,80 @@ __device__ __forceinline__ void linear4_impl(const qw_linear4_args &a) {
                                                       sum[c][t][r]);
             }
         }
-    }
-    /* the waves' sums meet in halves: rows 4 g + r of tile t, column i */
+    };
+    /* slabs at, at + 1 (one a set) from buffer, weights of the two pairs after
+     * in flight */
+    load_x(first);
+    load_w(0, first + set);
+    load_w(1, first + 2 + set);
+    store_x(0);
+    load_x(first + 2);
+    __syncthreads();
+    uint32_t buffer = 0;
+    for (uint32_t at = first; at < last; at += 4) {
 #pragma unroll
-    for (uint32_t h = L4_WAVES / 2; h > 0; h >>= 1) {
-        if (wave >= h && wave < 2 * h) {
-#pragma unroll
-            for (int c = 0; c < CT; c++)
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-                    *(floatx4 *)&part[wave - h][(c * NT + t) * 256 + lane * 4] = sum[c][t];
+        for (int u = 0; u < 2; u++) {
+            const uint32_t s = at + 2 * u; /* the same for all waves */
+            if (s >= last) break;
+            if (s + set < last) step(u, buffer, (s + set) * 128);
+            load_w(u, s + 4 + set);
+            if (s + 2 < last) {
+                store_x(buffer ^ 1);
+                load_x(s + 4);
+            }
+            __syncthreads();
+            buffer ^= 1;
         }
-        __syncthreads();
-        if (wave < h) {
-#pragma unroll
-            for (int c = 0; c < CT; c++)
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-                    sum[c][t] += *(const floatx4 *)&part[wave][(c * NT + t) * 256 + lane * 4];
-        }
-        __syncthreads();
     }
-    if (wave) return;
+    /* the second set's sums to the first: 4 waves x 2 NT KB */
+    float *meet = (float *)lds + (wave & 3) * (CT * NT * 256);
+    static_assert(4 * CT * NT * 1024 <= sizeof(lds), "");
+    if (set) {
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) *(floatx4 *)(meet + (c * NT + t) * 256 + lane * 4) = sum[c][t];
+    }
+    __syncthreads();
+    if (!set) {
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) sum[c][t] += *(const floatx4 *)(meet + (c * NT + t) * 256 + lane * 4);
+    }
+    if (a.pieces > 1) {
+        constexpr uint32_t PB = 4 * CT * NT * 1024; /* bytes of a piece */
+        const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)((unsigned char *)a.part + (size_t)tile * a.pieces * PB), (short)0,
+            (int)(a.pieces * PB), 0x00020000);
+        const uint32_t at = (wave & 3) * (CT * NT * 1024) + lane * 16;
+        if (!set) {
+#pragma unroll
+            for (int n = 0; n < CT * NT; n++)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum[n / NT][n % NT]), pr,
+                                                       piece * PB + at + n * 1024, 0, 17);
+            __builtin_amdgcn_s_waitcnt(0x0F70); /* vmcnt(0): the piece's stores are done */
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        __syncthreads();
+        if (tid == 0)
+            arrived = __hip_atomic_fetch_add(a.flag + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (arrived != a.pieces - 1) return;
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+        if (!set) {
+#pragma unroll
+            for (int n = 0; n < CT * NT; n++) sum[n / NT][n % NT] = floatx4{0, 0, 0, 0};
+            for (uint32_t pc = 0; pc < a.pieces; pc++)
+#pragma unroll
+                for (int n = 0; n < CT * NT; n++)
+                    sum[n / NT][n % NT] += __builtin_bit_cast(
+                        floatx4, __builtin_amdgcn_raw_buffer_load_b128(pr, pc * PB + at + n * 1024, 0, 17));
+        }
+        if (tid == 0)
+            __hip_atomic_store(a.flag + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (set) return;
 #pragma unroll
     for (int c = 0; c < CT; c++) {
         if (col0 + 16 * c + i >= a.cols) continue;
@@ -155,14 +375,16 @@ __device__ __forceinline__ void linear4_impl(const qw_linear4_args &a) {
             }
     }
 }
-#define L4_KERNEL(nt, ct, gs)                                                                \
-    QW_KERNEL void __launch_bounds__(64 * L4_WAVES, 2) qw_linear4_r##nt##c##ct##g##gs(qw_linear4_args a) { \
-        linear4_impl<nt, ct, gs>(a);                                                         \
+#define L4_MANY(nt, gs)                                                                        \
+    QW_KERNEL void __launch_bounds__(512, 2) qw_linear4_r##nt##_g##gs(qw_linear4_args a) {     \
+        linear4_many<nt, gs, false>(a);                                                        \
+    }                                                                                          \
+    QW_KERNEL void __launch_bounds__(512, 2) qw_linear4_r##nt##_g##gs##z(qw_linear4_args a) {  \
+        linear4_many<nt, gs, true>(a);                                                         \
     }
-#define L4_GROUPS(nt, ct) L4_KERNEL(nt, ct, 32) L4_KERNEL(nt, ct, 64) L4_KERNEL(nt, ct, 128)
-L4_GROUPS(1, 1)
-L4_GROUPS(2, 1)
-L4_GROUPS(4, 1)
+L4_MANY(1, 32) L4_MANY(1, 64) L4_MANY(1, 128)
+L4_MANY(2, 32) L4_MANY(2, 64) L4_MANY(2, 128)
+L4_MANY(4, 32) L4_MANY(4, 64) L4_MANY(4, 128)
 
 /* One wave per 64 groups' worth of weights would waste lanes on short rows, so
  * a lane has a group of its own: two passes over its 32 to 128 weights (the

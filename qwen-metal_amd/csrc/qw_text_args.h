@@ -48,6 +48,9 @@ typedef struct {
     const uint8_t *weight;
     const uint16_t *scales, *zeros, *bias;
     uint32_t rows, k, cols, lda, ldc;
+    uint32_t pieces; /* ranges of k that meet in part, counted in flag */
+    float *part;
+    uint32_t *flag;
 } qw_linear4_args;
 
 typedef struct {
