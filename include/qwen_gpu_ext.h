@@ -332,7 +332,7 @@ enum { QW_ROTARY_INTERLEAVED = 0, QW_ROTARY_HALF = 1 };
  * q_out may be q (the same rows, in place) and k_out k; otherwise outputs and
  * inputs do not overlap. heads or kv_heads may be 0 (without a cache): then
  * nothing is done for q or k. head_dim 64, 128 or 256; rotary_dim even, up to
- * head_dim. Rows are 16-byte aligned. */
+ * head_dim. Rows and norm weights are 16-byte aligned. */
 typedef struct {
     h3_gpu_tensor *q_out;
     size_t q_out_offset;
@@ -391,7 +391,8 @@ int qw_gpu_paged_attention_check(const qw_paged_attention_desc *desc, char *erro
  * input k of column c (the low half of byte k / 2 for even k), s = scales[c][k /
  * group] and z = zeros[c][k / group], 8 without zeros. Rows of in and out at
  * strides lda and ldc. fp32 sums, one rounding. group 32, 64 or 128; k a
- * multiple of it; cols of 8. The output overlaps no operand. */
+ * multiple of it; cols of 8. Rows of in are 16-byte aligned, of out 8, the
+ * weight 16, scales and zeros 4. The output overlaps no operand. */
 typedef struct {
     h3_gpu_tensor *out;
     size_t out_offset;

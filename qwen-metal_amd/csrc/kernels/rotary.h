@@ -10,7 +10,8 @@
  * once, at the store.
  *
  * Bound by HBM for many rows, by latency for few. A workgroup has one row and
- * 256 / (head_dim / 8) of its heads, a lane 16 bytes: the row's sines are made
+ * 256 / (head_dim / 8) of its heads (or three times as many), a lane 16 bytes
+ * of a head: the row's sines are made
  * once per workgroup and shared through LDS (made by every lane for itself
  * they cost 8 pairs for each 16 bytes, more than the bytes' time). */
 #pragma once
@@ -42,40 +43,49 @@ __device__ __forceinline__ uint32_t rotary_sequence(const qw_cache_args &c, uint
     return n;
 }
 
-template <int D>
+/* H heads a lane: 1 for few rows, where the chain of loads to a row's page is
+ * the time, 3 for many, where a row's chain, sines and norm weights serve 3
+ * times the bytes. */
+template <int D, int H>
 __device__ __forceinline__ void rotary_impl(const qw_rotary_args &a) {
-    constexpr uint32_t LPH = D / 8; /* lanes per head */
-    __shared__ qw_f2 turned[D / 2];
-    const uint32_t tid = threadIdx.x, row = blockIdx.x;
-    const uint32_t head = blockIdx.y * (256 / LPH) + tid / LPH, c8 = tid % LPH * 8;
+    constexpr uint32_t LPH = D / 8, HPP = 256 / LPH; /* lanes per head, heads per pass */
+    __shared__ __attribute__((aligned(16))) qw_f2 turned[D / 2];
+    const uint32_t tid = threadIdx.x, row = blockIdx.x, c8 = tid % LPH * 8;
+    const uint32_t head0 = blockIdx.y * (HPP * H) + tid / LPH;
     const uint32_t all = a.heads + a.kv_heads * (a.cached ? 2 : 1);
-    const bool live = head < all;
-    const bool is_q = head < a.heads, is_k = !is_q && head < a.heads + a.kv_heads;
-    const uint32_t kvh = is_q ? 0 : is_k ? head - a.heads : head - a.heads - a.kv_heads;
-    const u16 *src = is_q   ? a.q + (size_t)row * a.ldq + head * D
-                     : is_k ? a.k + (size_t)row * a.ldk + kvh * D
-                            : a.v + (size_t)row * a.ldv + kvh * D;
-    /* the row's own values, and those that they are paired with */
     const uint32_t hn = a.rotary_dim / 2;
-    const bool turns = live && (is_q || is_k), pairs = turns && a.half && c8 < a.rotary_dim;
-    u32x4 own = {0, 0, 0, 0}, other = {0, 0, 0, 0};
-    if (live) own = *(const u32x4 *)(src + c8);
-    /* element e pairs with e + hn below hn and e - hn from there on */
     const bool whole = hn % 8 == 0; /* a lane's partners lie in one chunk */
-    if (pairs && whole) other = *(const u32x4 *)(src + (c8 < hn ? c8 + hn : c8 - hn));
-    if (pairs && !whole) {
-        u16 t[8];
+    const bool pairs = a.half && c8 < a.rotary_dim;
+    /* each head's own values, and those that they are paired with: element e
+     * with e + hn below hn and e - hn from there on */
+    u32x4 own[H], other[H];
 #pragma unroll
-        for (uint32_t i = 0; i < 8; i++) {
-            const uint32_t e = c8 + i;
-            t[i] = e < hn ? src[e + hn] : e < a.rotary_dim ? src[e - hn] : 0;
+    for (int n = 0; n < H; n++) {
+        const uint32_t head = head0 + n * HPP;
+        own[n] = other[n] = u32x4{0, 0, 0, 0};
+        if (head >= all) continue;
+        const bool is_q = head < a.heads, is_k = head < a.heads + a.kv_heads;
+        const u16 *src = is_q   ? a.q + (size_t)row * a.ldq + head * D
+                         : is_k ? a.k + (size_t)row * a.ldk + (head - a.heads) * D
+                                : a.v + (size_t)row * a.ldv + (head - a.heads - a.kv_heads) * D;
+        own[n] = *(const u32x4 *)(src + c8);
+        if (!pairs || !is_k) continue;
+        if (whole) {
+            other[n] = *(const u32x4 *)(src + (c8 < hn ? c8 + hn : c8 - hn));
+        } else {
+            u16 t[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                const uint32_t e = c8 + i;
+                t[i] = e < hn ? src[e + hn] : e < a.rotary_dim ? src[e - hn] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) other[n][i] = t[2 * i] | (uint32_t)t[2 * i + 1] << 16;
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++) other[i] = t[2 * i] | (uint32_t)t[2 * i + 1] << 16;
     }
 
     uint32_t pos = 0;
-    uint64_t at = ~0ull; /* of the cache */
+    uint64_t at = ~0ull; /* of the cache's K/V head 0 */
     if (a.cached) {
         const uint32_t s = rotary_sequence(a.cache, row);
         if (s == a.cache.sequences) return; /* behind the last sequence */
@@ -85,7 +95,7 @@ __device__ __forceinline__ void rotary_impl(const qw_rotary_args &a) {
         if (place < 0) return; /* a token that its sequence does not have */
         pos = (uint32_t)place;
         const uint32_t page = a.cache.table[qw_cache_entry(a.cache, s, pos)];
-        if (page < a.cache.pages) at = qw_cache_at(a.cache, page, pos, kvh, D);
+        if (page < a.cache.pages) at = qw_cache_at(a.cache, page, pos, 0, D);
     }
     if (a.positions) pos = a.positions[row];
     if (tid < hn) {
@@ -94,61 +104,76 @@ __device__ __forceinline__ void rotary_impl(const qw_rotary_args &a) {
         turned[tid] = qw_f2{cs[0] * a.factor, cs[1] * a.factor};
     }
     __syncthreads();
-    if (!live) return;
-
-    if (turns) {
-        float x[8], y[8];
+    /* the lane's sines, the same for all its heads: y = x c + other s, the sign
+     * of s by the side */
+    float c[8], s[8];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[2 * i] = lo_bf(own[i]), x[2 * i + 1] = hi_bf(own[i]);
-            y[2 * i] = lo_bf(other[i]), y[2 * i + 1] = hi_bf(other[i]);
-        }
-        const u16 *w = is_q ? a.norm_q : a.norm_k;
-        if (w) {
-            float s = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) s = __builtin_fmaf(x[i], x[i], s);
-#pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-            const float inv = __builtin_amdgcn_rsqf(__builtin_fmaf(s, 1.0f / D, a.eps));
-#pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
-                const uint32_t e = c8 + i;
-                x[i] *= inv * bf2f(w[e]);
-                if (pairs && e < a.rotary_dim) y[i] *= inv * bf2f(w[e < hn ? e + hn : e - hn]);
-            }
-        }
-        float z[8];
-#pragma unroll
-        for (uint32_t i = 0; i < 8; i++) z[i] = x[i];
-        if (a.half) {
-#pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
-                const uint32_t e = c8 + i;
-                if (e >= a.rotary_dim) continue;
-                const qw_f2 t = turned[e < hn ? e : e - hn];
-                z[i] = e < hn ? x[i] * t[0] - y[i] * t[1] : y[i] * t[1] + x[i] * t[0];
-            }
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < 8; i += 2) {
-                if (c8 + i >= a.rotary_dim) continue;
-                const qw_f2 t = turned[(c8 + i) / 2];
-                z[i] = x[i] * t[0] - x[i + 1] * t[1];
-                z[i + 1] = x[i] * t[1] + x[i + 1] * t[0];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) own[i] = pack_bf(z[2 * i], z[2 * i + 1]);
+    for (uint32_t i = 0; i < 8; i++) {
+        const uint32_t e = c8 + i;
+        c[i] = 1.0f, s[i] = 0.0f;
+        if (e >= a.rotary_dim) continue;
+        const qw_f2 t = turned[!a.half ? e / 2 : e < hn ? e : e - hn];
+        c[i] = t[0];
+        s[i] = (a.half ? e < hn : !(e & 1)) ? -t[1] : t[1];
     }
-    if (is_q) {
-        *(u32x4 *)(a.q_out + (size_t)row * a.ldq_out + head * D + c8) = own;
-    } else if (!a.cached) {
-        *(u32x4 *)(a.k_out + (size_t)row * a.ldk_out + kvh * D + c8) = own;
-    } else if (at != ~0ull) {
-        *(u32x4 *)((is_k ? a.cache.k : a.cache.v) + at + c8) = own;
+#pragma unroll
+    for (int n = 0; n < H; n++) {
+        const uint32_t head = head0 + n * HPP;
+        if (head >= all) continue;
+        const bool is_q = head < a.heads, is_k = !is_q && head < a.heads + a.kv_heads;
+        const uint32_t kvh = is_q ? 0 : is_k ? head - a.heads : head - a.heads - a.kv_heads;
+        if (is_q || is_k) {
+            float x[8], y[8];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                x[2 * i] = lo_bf(own[n][i]), x[2 * i + 1] = hi_bf(own[n][i]);
+                y[2 * i] = lo_bf(other[n][i]), y[2 * i + 1] = hi_bf(other[n][i]);
+            }
+            const u16 *w = is_q ? a.norm_q : a.norm_k;
+            if (w) {
+                float sq = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) sq = __builtin_fmaf(x[i], x[i], sq);
+#pragma unroll
+                for (int o = LPH / 2; o > 0; o >>= 1) sq += __shfl_xor(sq, o, 64);
+                const float inv = __builtin_amdgcn_rsqf(__builtin_fmaf(sq, 1.0f / D, a.eps));
+                const u32x4 wv = *(const u32x4 *)(w + c8);
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[2 * i] *= inv * lo_bf(wv[i]), x[2 * i + 1] *= inv * hi_bf(wv[i]);
+                if (pairs && whole) {
+                    const u32x4 ov = *(const u32x4 *)(w + (c8 < hn ? c8 + hn : c8 - hn));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y[2 * i] *= inv * lo_bf(ov[i]), y[2 * i + 1] *= inv * hi_bf(ov[i]);
+                } else if (pairs) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; i++) {
+                        const uint32_t e = c8 + i;
+                        if (e < a.rotary_dim) y[i] *= inv * bf2f(w[e < hn ? e + hn : e - hn]);
+                    }
+                }
+            }
+            if (!a.half) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) y[i] = x[i ^ 1];
+            }
+            /* past rotary_dim c = 1, s = 0 and y = 0 or a finite neighbour's:
+             * only there could an infinity in y spoil x, so it is left out */
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (c8 + i < a.rotary_dim) x[i] = __builtin_fmaf(y[i], s[i], x[i] * c[i]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) own[n][i] = pack_bf(x[2 * i], x[2 * i + 1]);
+        }
+        if (is_q) {
+            *(u32x4 *)(a.q_out + (size_t)row * a.ldq_out + head * D + c8) = own[n];
+        } else if (!a.cached) {
+            *(u32x4 *)(a.k_out + (size_t)row * a.ldk_out + kvh * D + c8) = own[n];
+        } else if (at != ~0ull) {
+            *(u32x4 *)((is_k ? a.cache.k : a.cache.v) + at + kvh * D + c8) = own[n];
+        }
     }
 }
-QW_KERNEL void __launch_bounds__(256) qw_rotary_d64(qw_rotary_args a) { rotary_impl<64>(a); }
-QW_KERNEL void __launch_bounds__(256) qw_rotary_d128(qw_rotary_args a) { rotary_impl<128>(a); }
-QW_KERNEL void __launch_bounds__(256) qw_rotary_d256(qw_rotary_args a) { rotary_impl<256>(a); }
+#define ROTARY(d)                                                                                     \
+    QW_KERNEL void __launch_bounds__(256) qw_rotary_d##d(qw_rotary_args a) { rotary_impl<d, 1>(a); }  \
+    QW_KERNEL void __launch_bounds__(256) qw_rotary_d##d##_h3(qw_rotary_args a) { rotary_impl<d, 3>(a); }
+ROTARY(64) ROTARY(128) ROTARY(256)
