@@ -35,11 +35,13 @@ __device__ __forceinline__ float attn_exp(const floatx16 (&s)[AKB], bf16x8 (&pf)
  * assembly so the compiler does not treat it as a pending LDS store (it
  * would wait for every one in flight before each LDS read); the kernel
  * waits for them itself (vmcnt) before the barrier that publishes a tile. The
- * load reads M0 one wait state after its write at the earliest (gfx9 rule;
- * the compiler does not see inside the asm to insert it). */
+ * load reads M0 one wait state after its write at the earliest, and a scalar
+ * register that a vector instruction wrote (a spilled one read back from a
+ * lane, a page's address) five after (gfx9 rules; the compiler does not see
+ * inside the asm to insert them): the write of M0 and s_nop 3. */
 __device__ __forceinline__ void attn_dma(u32x4 rsrc, uint32_t lds_base, uint32_t voff,
                                          uint32_t soff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(lds_base), "v"(voff), "s"(rsrc), "s"(soff)
                  : "m0");

@@ -20,6 +20,8 @@ branches), the wait states between:
   mfma->write  an MFMA result and a VALU write of the same register: passes + 3
   srcc->write  an MFMA reading a register as srcC and a VALU write of it: passes
   m0->lds      an SALU write of M0 and an LDS-direct load (``... lds``): 1
+  vsgpr->lds   a VALU write of a scalar register (readlane, readfirstlane) and
+               an LDS-direct load that reads it: 5
 
 (``s_nop N`` counts N + 1 wait states, every other instruction 1; passes
 as counted here: 4x4 2, 16x16 8, 32x32 16. These are upper bounds: for its
@@ -31,7 +33,7 @@ destination as srcC with the same register range chains in hardware and
 needs none. Exit status 1 and
 a listing when any distance is short.
 
-``--lds-only`` reports the m0->lds distance alone: for a code object whose
+``--lds-only`` reports the distances to LDS-direct loads alone: for a code object whose
 matrix instructions are all builtins, which the compiler spaces by its own,
 exact tables (the text kernels, where only the LDS-direct loads are inline
 assembly).
@@ -50,6 +52,7 @@ LLVM = os.path.join(ROCM, "llvm", "bin")
 VALU_WRITE_TO_MFMA = 2
 MFMA_EXTRA = 3
 M0_TO_LDS_DMA = 1
+VALU_SGPR_TO_LDS_DMA = 5
 
 
 def _regs(tok):
@@ -60,6 +63,14 @@ def _regs(tok):
     if m:
         return {(m.group(1), int(m.group(2)))}
     return set()
+
+
+def _sregs(tok):
+    m = re.fullmatch(r"s\[(\d+):(\d+)\]", tok)
+    if m:
+        return set(range(int(m.group(1)), int(m.group(2)) + 1))
+    m = re.fullmatch(r"s(\d+)", tok)
+    return {int(m.group(1))} if m else set()
 
 
 def _passes(op):
@@ -74,7 +85,7 @@ def _passes(op):
 
 class Insn:
     __slots__ = ("addr", "text", "op", "ops", "nws", "dst", "srcs", "mfma", "m0w",
-                 "lds_dma", "succ", "pred", "valu_write")
+                 "lds_dma", "succ", "pred", "valu_write", "valu_sgpr", "sgprs")
 
     def __init__(self, addr, text):
         self.addr, self.text = addr, text
@@ -104,6 +115,11 @@ class Insn:
         self.m0w = op.startswith("s_") and bool(self.ops) and self.ops[0] == "m0"
         self.lds_dma = (op.startswith(("buffer_load", "global_load")) and
                         re.search(r"\slds(\s|$)", text) is not None)
+        # scalar registers that a vector instruction writes (readlane,
+        # readfirstlane, compares), and those that this instruction names
+        self.valu_sgpr = (_sregs(self.ops[0]) if op.startswith("v_") and not self.mfma and
+                          self.ops else set())
+        self.sgprs = set().union(*[_sregs(t) for t in self.ops]) if self.ops else set()
         self.succ, self.pred = [], []
 
 
@@ -205,6 +221,9 @@ def check(funcs):
                 if x.lds_dma:
                     for ws, y in _back(x, M0_TO_LDS_DMA, lambda y: y.m0w):
                         bad.append((name, "m0->lds", ws, M0_TO_LDS_DMA, y, x))
+                    for ws, y in _back(x, VALU_SGPR_TO_LDS_DMA,
+                                       lambda y: y.valu_sgpr & x.sgprs):
+                        bad.append((name, "vsgpr->lds", ws, VALU_SGPR_TO_LDS_DMA, y, x))
     return bad
 
 
@@ -216,7 +235,7 @@ def main(argv):
     funcs = functions(disassemble(argv[1]))
     bad = check(funcs)
     if "--lds-only" in argv:
-        bad = [b for b in bad if b[1] == "m0->lds"]
+        bad = [b for b in bad if b[1].endswith("->lds")]
     n = sum(len(v) for v in funcs.values())
     if not bad:
         print("hazard_check: %d instructions in %d kernels, no short distances" % (n, len(funcs)))
