@@ -77,11 +77,12 @@ __device__ __forceinline__ void pa_limits(const qw_paged_args &a, const qw_span 
     lo = a.window && hi > a.window ? hi - a.window : 0;
 }
 
-/* Buffer of one load's keys: `n` tokens from t on, those below `end`. */
-__device__ __forceinline__ u32x4 pa_rsrc(const qw_cache_args &c, const u16 *base, uint32_t page,
-                                         uint32_t t, uint32_t n, uint32_t end, uint32_t head) {
+/* Buffer of one load's keys: `n` tokens from t on, those below `end`, of the
+ * head whose first element is at `base`. */
+__device__ __forceinline__ u32x4 pa_rsrc(const qw_cache_args &c, uint64_t base, uint32_t page,
+                                         uint32_t t, uint32_t n, uint32_t end) {
     const bool there = page < c.pages;
-    const uint64_t at = (uint64_t)(base + qw_cache_at(c, there ? page : 0, t, head, PA_D));
+    const uint64_t at = base + 2 * qw_cache_at(c, there ? page : 0, t, 0, PA_D);
     const uint32_t bytes = qw_cache_bytes(c, t, n, end, PA_D);
     /* the same in every lane: said so, or the compiler keeps it in vector registers */
     return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at),
@@ -96,6 +97,11 @@ __device__ __forceinline__ uint64_t pa_seen(uint32_t kv0, uint32_t lo, uint32_t 
     const uint64_t below = n < 64 ? (1ull << n) - 1 : ~0ull;
     return skip < 64 ? have & below & (~0ull << skip) : 0;
 }
+/* v where bit b of m is set, else -inf: two instructions (bit field, insert) */
+__device__ __forceinline__ float pa_where(uint32_t m, int b, float v) {
+    const uint32_t all = (uint32_t)__builtin_amdgcn_sbfe((int)m, b, 1);
+    return __uint_as_float((all & __float_as_uint(v)) | (~all & 0xff800000u));
+}
 /* Key of s[kbk][v] in a tile: 32 kbk + 8 (v / 4) + 4 h + v % 4; seen: bits of
  * the keys, moved down by 4 h. */
 __device__ __forceinline__ void pa_mask(floatx16 (&s)[AKB], uint64_t seen) {
@@ -104,17 +110,21 @@ __device__ __forceinline__ void pa_mask(floatx16 (&s)[AKB], uint64_t seen) {
     for (int kbk = 0; kbk < AKB; kbk++)
 #pragma unroll
         for (int v = 0; v < 16; v++)
-            if (!(half[kbk] & 1u << (8 * (v >> 2) + (v & 3)))) s[kbk][v] = -INFINITY;
+            s[kbk][v] = pa_where(half[kbk], 8 * (v >> 2) + (v & 3), s[kbk][v]);
 }
 
-/* One of 8 bf16 values is infinite or NaN. */
-__device__ __forceinline__ bool pa_not_finite(bf16x8 v) {
+/* The greatest magnitudes, as bit patterns, of 8 bf16 values and those of m, in
+ * pairs; 0x7f80 or more in a half: one is infinite or NaN. */
+typedef u16 u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2 pa_greatest(u16x2 m, bf16x8 v) {
     const u32x4 w = __builtin_bit_cast(u32x4, v);
-    bool bad = false;
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        bad |= (w[i] & 0x7f800000u) == 0x7f800000u || (w[i] & 0x7f80u) == 0x7f80u;
-    return bad;
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+    return m;
+}
+__device__ __forceinline__ bool pa_not_finite(u16x2 m) {
+    return __builtin_amdgcn_ballot_w64(m[0] >= 0x7f80 || m[1] >= 0x7f80) != 0;
 }
 /* v with zeros in place of what is not finite */
 __device__ __forceinline__ bf16x8 pa_finite(bf16x8 v) {
@@ -245,6 +255,7 @@ __device__ __forceinline__ void pa_again(const qw_paged_args &a, const pa_job &j
     }
 }
 
+#define PM_PIECES 8 /* at most */
 /* NW waves of 32 rows. Pieces: a block's key tiles are cut in a.pieces ranges
  * that meet in memory as the image attention's do. */
 template <int NW, bool SPLIT>
@@ -298,33 +309,62 @@ __device__ __forceinline__ void pa_many(const qw_paged_args &a) {
     }
     /* a tile's table entries, one key a lane, and the page ids they give; no
      * page: 0xffffffff */
+    const uint32_t *const table = a.cache.table + (size_t)job.seq * a.cache.table_ld;
     auto entry = [&](uint32_t kv0) __attribute__((always_inline)) {
-        return a.cache.table[qw_cache_entry(a.cache, job.seq, kv0 + lane)];
+        return table[min((kv0 + lane) >> a.cache.page_shift, a.cache.table_ld - 1)];
     };
     auto page_of = [&](uint32_t p, uint32_t kv0) __attribute__((always_inline)) {
         return kv0 + lane < hi_last && p < a.cache.pages ? p : 0xffffffffu;
     };
-    auto issue = [&](const u16 *base, uint32_t stage, uint32_t kv0, uint32_t ids,
-                     const uint32_t (&off)[DPW]) __attribute__((always_inline)) {
+    const uint64_t kbase = (uint64_t)(a.cache.k + kvh * PA_D), vbase = (uint64_t)(a.cache.v + kvh * PA_D);
+    const uint32_t token_bytes = ld * 2, slots = (1u << a.cache.page_shift) - 1;
+    /* a whole tile's loads: byte offsets of their keys in K and V, in a few
+     * scalar instructions each */
+    auto places = [&](uint64_t (&at)[DPW], uint32_t kv0, uint32_t ids) __attribute__((always_inline)) {
+#pragma unroll
+        for (int jj = 0; jj < DPW; jj++) {
+            const uint32_t blk = wave * DPW + jj, page = __builtin_amdgcn_readlane(ids, blk * 4);
+            at[jj] = (uint64_t)((page << a.cache.page_shift) + ((kv0 + 4 * blk) & slots)) * token_bytes;
+        }
+    };
+    auto issue = [&](uint64_t base, uint32_t stage, uint32_t kv0, uint32_t ids, uint64_t have,
+                     const uint64_t (&at)[DPW], const uint32_t (&off)[DPW]) __attribute__((always_inline)) {
+        if (have == ~0ull) {
+#pragma unroll
+            for (int jj = 0; jj < DPW; jj++)
+                attn_dma(u32x4{(uint32_t)(base + at[jj]), (uint32_t)((base + at[jj]) >> 32) & 0xffffu,
+                               3 * token_bytes + 2 * PA_D, 0x00020000u},
+                         lds0 + stage * A_TILE + (wave * DPW + jj) * 1024, off[jj], 0);
+            return;
+        }
 #pragma unroll
         for (int jj = 0; jj < DPW; jj++) {
             const uint32_t blk = wave * DPW + jj;
             const uint32_t page = __builtin_amdgcn_readlane(ids, blk * 4);
-            attn_dma(pa_rsrc(a.cache, base, page, kv0 + 4 * blk, 4, hi_last, kvh),
+            attn_dma(pa_rsrc(a.cache, base, page, kv0 + 4 * blk, 4, hi_last),
                      lds0 + stage * A_TILE + blk * 1024, off[jj], 0);
         }
     };
-    /* page ids of tiles t and t + 1, and tile t + 2's entries, which were
-     * asked for a tile ahead */
-    uint32_t id0 = 0xffffffffu, id1 = 0xffffffffu, next = 0;
+    /* page ids of tiles t and t + 1, which of their keys have one and where
+     * their loads are, and tile t + 2's entries, which were asked for a tile
+     * ahead */
+    uint32_t id1 = 0xffffffffu, next = 0;
+    uint64_t have0 = 0, have1 = 0, at1[DPW];
+#pragma unroll
+    for (int jj = 0; jj < DPW; jj++) at1[jj] = 0;
     if (ntiles) {
         const uint32_t e0 = entry(tile0 * AKT), e1 = entry((tile0 + 1) * AKT);
         next = entry((tile0 + 2) * AKT);
-        id0 = page_of(e0, tile0 * AKT);
+        const uint32_t id0 = page_of(e0, tile0 * AKT);
         id1 = page_of(e1, (tile0 + 1) * AKT);
-        issue(a.cache.k, 0, tile0 * AKT, id0, kvo);
-        issue(a.cache.v, 2, tile0 * AKT, id0, vvo);
-        issue(a.cache.k, 1, (tile0 + 1) * AKT, id1, kvo);
+        have0 = __builtin_amdgcn_ballot_w64(id0 != 0xffffffffu);
+        have1 = __builtin_amdgcn_ballot_w64(id1 != 0xffffffffu);
+        uint64_t at0[DPW];
+        places(at0, tile0 * AKT, id0);
+        places(at1, (tile0 + 1) * AKT, id1);
+        issue(kbase, 0, tile0 * AKT, id0, have0, at0, kvo);
+        issue(vbase, 2, tile0 * AKT, id0, have0, at0, vvo);
+        issue(kbase, 1, (tile0 + 1) * AKT, id1, have1, at1, kvo);
     }
     bf16x8 qf[8];
     {
@@ -371,20 +411,23 @@ __device__ __forceinline__ void pa_many(const qw_paged_args &a) {
         constexpr uint32_t st = decltype(odd)::value;
         const uint32_t kv0 = (tile0 + t) * AKT;
         const uint32_t id2 = page_of(next, kv0 + 2 * AKT);
-        issue(a.cache.k, st, kv0 + 2 * AKT, id2, kvo);
-        issue(a.cache.v, 2 + (st ^ 1), kv0 + AKT, id1, vvo);
+        const uint64_t have2 = __builtin_amdgcn_ballot_w64(id2 != 0xffffffffu);
+        uint64_t at2[DPW];
+        places(at2, kv0 + 2 * AKT, id2);
+        issue(kbase, st, kv0 + 2 * AKT, id2, have2, at2, kvo);
+        issue(vbase, 2 + (st ^ 1), kv0 + AKT, id1, have1, at1, vvo);
+#pragma unroll
+        for (int jj = 0; jj < DPW; jj++) at1[jj] = at2[jj];
         next = entry(kv0 + 3 * AKT);
-        /* keys of this tile without a page */
-        const uint64_t have = __builtin_amdgcn_ballot_w64(id0 != 0xffffffffu);
-        const bool masked = kv0 + AKT > hi_least || kv0 < lo_most || have != ~0ull;
+        const bool masked = kv0 + AKT > hi_least || kv0 < lo_most || have0 != ~0ull;
         if (masked) {
-            pa_mask(sc, pa_seen(kv0, lo, L, have) >> 4 * h);
+            pa_mask(sc, pa_seen(kv0, lo, L, have0) >> 4 * h);
             const unsigned char *vs = lds + (2 + st) * A_TILE;
-            bool bad = false;
-#pragma unroll 2
+            u16x2 most = {0, 0};
+#pragma unroll 4
             for (uint32_t n = 0; n < A_TILE / 1024; n++)
-                bad |= pa_not_finite(*(const bf16x8 *)(vs + n * 1024 + lane * 16));
-            odd_values |= __builtin_amdgcn_ballot_w64(bad) != 0;
+                most = pa_greatest(most, *(const bf16x8 *)(vs + n * 1024 + lane * 16));
+            odd_values |= pa_not_finite(most);
         }
         bf16x8 vpre[4];
 #pragma unroll
@@ -427,7 +470,7 @@ __device__ __forceinline__ void pa_many(const qw_paged_args &a) {
             for (int db = 0; db < 4; db++)
                 o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tk ? read_v(st, tk, db) : vpre[db],
                                                                 pf[tk], o[db], 0, 0, 0);
-        id0 = id1, id1 = id2;
+        id1 = id2, have0 = have1, have1 = have2;
         __builtin_amdgcn_s_waitcnt(0x0F70); /* vmcnt(0): K(t + 2), V(t + 1) landed */
         attn_barrier();
     };
@@ -463,33 +506,53 @@ __device__ __forceinline__ void pa_many(const qw_paged_args &a) {
         __syncthreads();
         if (arrived != pieces - 1) return;
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-        float m_all = -INFINITY;
-        for (uint32_t pc = 0; pc < pieces; pc++)
-            m_all = fmaxf(m_all, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                                     pr, pc * PB + wave * WB + 16 * 1024 + lane * 4, 0, 17)));
+        /* Every load here takes memory's latency, so all pieces' m and l are
+         * asked for together, and O two pieces at a time. A piece in which the
+         * row sees no key has m = -inf, O = l = 0; so has a piece past the
+         * last, read as it with the factor 0. */
+        float f[PM_PIECES], m_all = -INFINITY;
+#pragma unroll
+        for (uint32_t pc = 0; pc < PM_PIECES; pc++)
+            f[pc] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                pr, min(pc, pieces - 1) * PB + wave * WB + 16 * 1024 + lane * 4, 0, 17));
+        float l[PM_PIECES];
+#pragma unroll
+        for (uint32_t pc = 0; pc < PM_PIECES; pc++)
+            l[pc] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                pr, min(pc, pieces - 1) * PB + wave * WB + 16 * 1024 + 256 + lane * 4, 0, 17));
+#pragma unroll
+        for (uint32_t pc = 0; pc < PM_PIECES; pc++) m_all = fmaxf(m_all, f[pc]);
+        l_run = 0.0f;
+#pragma unroll
+        for (uint32_t pc = 0; pc < PM_PIECES; pc++) {
+            f[pc] = f[pc] == -INFINITY || pc >= pieces ? 0.0f : __builtin_amdgcn_exp2f(f[pc] - m_all);
+            l_run = __builtin_fmaf(l[pc], f[pc], l_run);
+        }
 #pragma unroll
         for (int db = 0; db < 4; db++)
 #pragma unroll
             for (int v = 0; v < 16; v++) o[db][v] = 0.0f;
-        l_run = 0.0f;
-        for (uint32_t pc = 0; pc < pieces; pc++) {
-            const uint32_t at = pc * PB + wave * WB;
-            const float m = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(pr, at + 16 * 1024 + lane * 4, 0, 17));
-            const float l = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(pr, at + 16 * 1024 + 256 + lane * 4, 0, 17));
-            floatx4 q[16];
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                q[i] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                       pr, at + i * 1024 + lane * 16, 0, 17));
-            /* a piece in which the row sees no key has m = -inf, O = l = 0 */
-            if (m == -INFINITY) continue;
-            const float f = __builtin_amdgcn_exp2f(m - m_all);
-            l_run = __builtin_fmaf(l, f, l_run);
+        for (uint32_t pc = 0; pc < PM_PIECES; pc += 2) {
+            if (pc >= pieces) break;
+            floatx4 q[2][16];
 #pragma unroll
-            for (int i = 0; i < 16; i++)
+            for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    o[i >> 2][4 * (i & 3) + e] = __builtin_fmaf(q[i][e], f, o[i >> 2][4 * (i & 3) + e]);
+                for (int i = 0; i < 16; i++)
+                    q[n][i] = __builtin_bit_cast(
+                        floatx4, __builtin_amdgcn_raw_buffer_load_b128(
+                                     pr, min(pc + n, pieces - 1) * PB + wave * WB + i * 1024 + lane * 16, 0, 17));
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        /* not a sum with 0 times an infinity */
+                        const float x = q[n][i][e], y = o[i >> 2][4 * (i & 3) + e];
+                        o[i >> 2][4 * (i & 3) + e] = f[pc + n] != 0.0f ? __builtin_fmaf(x, f[pc + n], y) : y;
+                    }
         }
         if (tid == 0)
             __hip_atomic_store(a.flag + place, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -510,7 +573,6 @@ __device__ __forceinline__ void pa_many(const qw_paged_args &a) {
                       pack_bf(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv)};
 }
 QW_KERNEL void __launch_bounds__(512, 1) qw_paged_attention_q256(qw_paged_args a) { pa_many<8, false>(a); }
-QW_KERNEL void __launch_bounds__(512, 1) qw_paged_attention_q256_split(qw_paged_args a) { pa_many<8, true>(a); }
 QW_KERNEL void __launch_bounds__(256, 2) qw_paged_attention_q128(qw_paged_args a) { pa_many<4, false>(a); }
 QW_KERNEL void __launch_bounds__(256, 2) qw_paged_attention_q128_split(qw_paged_args a) { pa_many<4, true>(a); }
 
@@ -570,20 +632,38 @@ __device__ __forceinline__ void pa_few(const qw_paged_args &a) {
      * fragment pass reads one chunk of 16 rows) and at c ^ 2 (k % 8) in V
      * tiles (a transposing pass reads 2 chunks of 8 rows) */
     const uint32_t drow = lane >> 4, dphys = lane & 15, ld = a.cache.kv_heads * PA_D;
+    uint32_t koff[4], voff[2];
+#pragma unroll
+    for (uint32_t n = 0; n < 4; n++) koff[n] = (drow * ld + ((dphys ^ (4 * n + drow)) * 8)) * 2;
+#pragma unroll
+    for (uint32_t n = 0; n < 2; n++) voff[n] = (drow * ld + ((dphys ^ (2 * (4 * n + drow))) * 8)) * 2;
+    const uint64_t kbase = (uint64_t)(a.cache.k + kvh * PA_D), vbase = (uint64_t)(a.cache.v + kvh * PA_D);
     uint32_t id0 = 0; /* table entry of ids[0] */
     bool gap = false; /* a page of the segment does not exist */
+    const uint32_t token_bytes = ld * 2, slots = (1u << a.cache.page_shift) - 1;
     auto issue = [&](uint32_t stage, uint32_t tile) __attribute__((always_inline)) {
+        const uint32_t to = lds0 + stage * 2 * PF_TILE;
+        /* the ids of the tile's keys, one a lane: one LDS read */
+        const uint32_t mine_ = tile * PF_KEYS + (lane & 31);
+        const uint32_t page_ = mine_ < hi_last ? ids[(mine_ >> a.cache.page_shift) - id0] : 0xffffffffu;
+        if (__builtin_amdgcn_ballot_w64(page_ != 0xffffffffu) == ~0ull) {
+#pragma unroll
+            for (int n = 0; n < PF_KEYS / 4; n++) {
+                const uint32_t page = __builtin_amdgcn_readlane(page_, 4 * n);
+                const uint64_t at = (uint64_t)((page << a.cache.page_shift) + ((tile * PF_KEYS + 4 * n) & slots)) * token_bytes;
+                const uint64_t k = kbase + at, v = vbase + at;
+                attn_dma(u32x4{(uint32_t)k, (uint32_t)(k >> 32) & 0xffffu, 3 * token_bytes + 2 * PA_D, 0x00020000u},
+                         to + n * 1024, koff[n & 3], 0);
+                attn_dma(u32x4{(uint32_t)v, (uint32_t)(v >> 32) & 0xffffu, 3 * token_bytes + 2 * PA_D, 0x00020000u},
+                         to + PF_TILE + n * 1024, voff[n & 1], 0);
+            }
+            return;
+        }
 #pragma unroll
         for (int n = 0; n < PF_KEYS / 4; n++) {
-            const uint32_t t = tile * PF_KEYS + 4 * n, row = 4 * n + drow;
-            uint32_t page = 0xffffffffu;
-            if (t < hi_last) page = ids[(t >> a.cache.page_shift) - id0];
-            page = __builtin_amdgcn_readfirstlane(page);
-            const uint32_t to = lds0 + stage * 2 * PF_TILE + n * 1024;
-            attn_dma(pa_rsrc(a.cache, a.cache.k, page, t, 4, hi_last, kvh), to,
-                     (drow * ld + ((dphys ^ (row & 15)) * 8)) * 2, 0);
-            attn_dma(pa_rsrc(a.cache, a.cache.v, page, t, 4, hi_last, kvh), to + PF_TILE,
-                     (drow * ld + ((dphys ^ (2 * (row & 7))) * 8)) * 2, 0);
+            const uint32_t t = tile * PF_KEYS + 4 * n, page = __builtin_amdgcn_readlane(page_, 4 * n);
+            attn_dma(pa_rsrc(a.cache, kbase, page, t, 4, hi_last), to + n * 1024, koff[n & 3], 0);
+            attn_dma(pa_rsrc(a.cache, vbase, page, t, 4, hi_last), to + PF_TILE + n * 1024, voff[n & 1], 0);
         }
     };
     const uint32_t te = i >> 2, tq = i & 3;
@@ -636,7 +716,7 @@ __device__ __forceinline__ void pa_few(const qw_paged_args &a) {
                 const uint32_t seen = (uint32_t)pa_seen(kv0, lo[rt], L[rt], have) >> 4 * g;
 #pragma unroll
                 for (int n = 0; n < 8; n++)
-                    if (!(seen & 1u << (16 * (n >> 2) + (n & 3)))) s[rt][n >> 2][n & 3] = -INFINITY;
+                    s[rt][n >> 2][n & 3] = pa_where(seen, 16 * (n >> 2) + (n & 3), s[rt][n >> 2][n & 3]);
             }
         }
         bf16x8 pf[RT];
@@ -678,10 +758,10 @@ __device__ __forceinline__ void pa_few(const qw_paged_args &a) {
         }
         bool odd_values = false;
         if (masked) {
-            bool bad = false;
+            u16x2 most = {0, 0};
 #pragma unroll
-            for (int db = 0; db < 8; db++) bad |= pa_not_finite(read_v(stage, db));
-            odd_values = __builtin_amdgcn_ballot_w64(bad) != 0;
+            for (int db = 0; db < 8; db++) most = pa_greatest(most, read_v(stage, db));
+            odd_values = pa_not_finite(most);
         }
         if (!odd_values) {
 #pragma unroll
@@ -780,6 +860,7 @@ __device__ __forceinline__ void pa_few(const qw_paged_args &a) {
                 acc[rt][e] = __builtin_fmaf(row[w * SUMS + (tid & 15) * 8 + e], f, acc[rt][e]);
         }
     }
+    uint32_t rows_left = rows; /* that this thread stores */
     if (used > 1) {
         /* a piece's rows [row][128 | m | l] in memory, as the waves' in LDS */
         float *part = a.part + (size_t)place * a.pieces * SUMS;
@@ -808,34 +889,79 @@ __device__ __forceinline__ void pa_few(const qw_paged_args &a) {
         __syncthreads();
         if (arrived != used - 1) return;
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+        /* All pieces' m and l come to LDS with one latency; then `sets` of
+         * threads take every sets-th piece of a row's 8 columns each, and meet
+         * in LDS. */
+        float *ml = (float *)lds; /* [row][piece][m | l], then a factor for m */
+        for (uint32_t e = tid; e < used * rows; e += 64 * PF_WAVES) {
+            const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(
+                pr, (e % used * SUMS + e / used * (PA_D + 4) + PA_D) * 4, 0, 17);
+            ml[2 * e] = __uint_as_float(v[0]), ml[2 * e + 1] = __uint_as_float(v[1]);
+        }
+        __syncthreads();
+        /* the rows' maxima and sums: 8 threads each */
+        float *total = ml + 2 * used * rows; /* [row] */
+        for (uint32_t r = tid / 8; r < rows; r += 8 * PF_WAVES) {
+            float m = -INFINITY, l = 0.0f;
+            for (uint32_t pc = tid & 7; pc < used; pc += 8) m = fmaxf(m, ml[2 * (r * used + pc)]);
+#pragma unroll
+            for (int o_ = 1; o_ < 8; o_ <<= 1) m = fmaxf(m, __shfl_xor(m, o_, 64));
+            for (uint32_t pc = tid & 7; pc < used; pc += 8) {
+                const float x = ml[2 * (r * used + pc)];
+                const float f = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m);
+                ml[2 * (r * used + pc)] = f;
+                l = __builtin_fmaf(ml[2 * (r * used + pc) + 1], f, l);
+            }
+#pragma unroll
+            for (int o_ = 1; o_ < 8; o_ <<= 1) l += __shfl_xor(l, o_, 64);
+            if ((tid & 7) == 0) total[r] = l;
+        }
+        __syncthreads();
+        float *meet = total + BM;
+        const uint32_t sets = rows > 8 ? 1 : rows > 4 ? 2 : 4, per = 16 * PF_WAVES / 4 / sets; /* rows a pass */
+        const uint32_t set = tid / 16 / per;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            const uint32_t row = 16 * rt + tid / 16;
-            if (row >= rows) continue;
-            const uint32_t at = row * (PA_D + 4) * 4;
-            float m_top = -INFINITY;
-            for (uint32_t pc = 0; pc < used; pc++)
-                m_top = fmaxf(m_top, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                                         pr, at + pc * SUMS * 4 + PA_D * 4, 0, 17)));
-            float l = 0.0f;
+            const uint32_t row = 16 * rt + tid / 16 % per;
 #pragma unroll
             for (int e = 0; e < 8; e++) acc[rt][e] = 0.0f;
-            for (uint32_t pc = 0; pc < used; pc++) {
-                const uint32_t from = at + pc * SUMS * 4;
-                const u32x2 ml = __builtin_amdgcn_raw_buffer_load_b64(pr, from + PA_D * 4, 0, 17);
-                const floatx4 q0 = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(pr, from + (tid & 15) * 32, 0, 17));
-                const floatx4 q1 = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(pr, from + (tid & 15) * 32 + 16, 0, 17));
-                const float m = __uint_as_float(ml[0]);
-                if (m == -INFINITY) continue;
-                const float f = __builtin_amdgcn_exp2f(m - m_top);
-                l = __builtin_fmaf(__uint_as_float(ml[1]), f, l);
+            if (row < rows) {
+                const uint32_t at = (row * (PA_D + 4) + (tid & 15) * 8) * 4;
+                for (uint32_t p0 = set; p0 < used; p0 += 4 * sets) {
+                    floatx4 q[4][2];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    acc[rt][e] = __builtin_fmaf(q0[e], f, acc[rt][e]);
-                    acc[rt][4 + e] = __builtin_fmaf(q1[e], f, acc[rt][4 + e]);
+                    for (int n = 0; n < 4; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            q[n][e] = __builtin_bit_cast(
+                                floatx4, __builtin_amdgcn_raw_buffer_load_b128(
+                                             pr, at + min(p0 + n * sets, used - 1) * SUMS * 4 + 16 * e, 0, 17));
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
+                        const uint32_t pc = p0 + n * sets;
+                        const float f = pc < used ? ml[2 * (row * used + pc)] : 0.0f;
+                        if (f == 0.0f) continue; /* no key of the row, or no such piece */
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            acc[rt][e] = __builtin_fmaf(q[n][e >> 2][e & 3], f, acc[rt][e]);
+                    }
+                }
+                l_all[rt] = total[row];
+                if (set) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        meet[((set - 1) * per + row) * PA_D + (tid & 15) * 8 + e] = acc[rt][e];
                 }
             }
-            l_all[rt] = l;
+        }
+        if (sets > 1) { /* at most 8 rows: RT's first tile alone */
+            __syncthreads();
+            if (set == 0 && tid / 16 < rows)
+                for (uint32_t n = 1; n < sets; n++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        acc[0][e] += meet[((n - 1) * per + tid / 16) * PA_D + (tid & 15) * 8 + e];
+            if (set) rows_left = 0;
         }
         if (tid == 0)
             __hip_atomic_store(a.flag + place, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -843,7 +969,7 @@ __device__ __forceinline__ void pa_few(const qw_paged_args &a) {
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const uint32_t row = 16 * rt + tid / 16;
-        if (row >= rows) continue;
+        if (row >= rows_left) continue;
         const uint32_t r = r0 + row, token = r / a.group, head = kvh * a.group + r % a.group;
         const float inv = l_all[rt] == 0.0f ? 0.0f : 1.0f / l_all[rt];
         u32x4 w;

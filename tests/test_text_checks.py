@@ -127,7 +127,8 @@ def test_rotary_without_cache(qd, memory):
     (dict(page_size=8192), "page_size"), (dict(pages=5), "too small"), (dict(pages=0), "no pages"),
     (dict(table_ld=4), "too small"), (dict(table_ld=1 << 28), "2^31"),
     (dict(sequences=3), "too small"), (dict(kv_heads=0), "no pages"), (dict(starts=None), "missing"),
-    (dict(pages=1 << 31, page_size=4096, kv_heads=1024, table_ld=1), "too small"),
+    (dict(pages=1 << 31, page_size=4096, kv_heads=1024, table_ld=1), "2^32"),
+    (dict(pages=(1 << 20) - 1, page_size=4096, kv_heads=1024, table_ld=1), "too small"),
 ])
 def test_cache_refusals(qd, memory, over, word):
     new = Maker(qd, memory)
