@@ -23,7 +23,10 @@
 #define L4_WAVES 8
 
 __device__ __forceinline__ bf16x8 l4_widen(uint32_t w) {
-    const uint32_t m = 0x000F000Fu, c = 0x43004300u;
+    /* one in a vector, one in a scalar register: v_and_or_b32 takes no literal,
+     * and the compiler's and, or with one each are two instructions */
+    uint32_t m = 0x000F000Fu, c = 0x43004300u;
+    asm("" : "+v"(m), "+s"(c));
     return __builtin_bit_cast(bf16x8, u32x4{(w & m) | c, (w >> 4 & m) | c, (w >> 8 & m) | c,
                                             (w >> 12 & m) | c});
 }
@@ -49,11 +52,25 @@ __device__ __forceinline__ u32x4 l4_transpose(u32x4 w) {
  * and the groups' scales and zero points (Z: there are some). Steps past the
  * last are read as it: no branch stands between a load and its use, where the
  * compiler would wait for every load. */
+template <int GS>
+using l4_pack = std::conditional_t<GS == 32, uint64_t, std::conditional_t<GS == 64, uint32_t, u16>>;
 template <int GS, bool Z>
 struct l4_step {
     u32x4 q;
-    u16 s[128 / GS], z[128 / GS];
+    l4_pack<GS> s, z; /* 16 bits a group */
 };
+/* 128 / GS neighbours of t[at], at most `count` in all, in one load (as single
+ * ones they took most of the time of small groups: 60 rows, 4096 -> 24576,
+ * groups of 32 with zero points 85 us -> .). Ones that would pass the end are
+ * read from it back and moved down. */
+template <int GS>
+__device__ __forceinline__ l4_pack<GS> l4_groups(const u16 *t, uint64_t at, uint64_t count) {
+    const uint64_t from = GS == 128 ? at : min(at, count - 128 / GS);
+    l4_pack<GS> v;
+    __builtin_memcpy(&v, t + from, sizeof(v));
+    if (GS < 128) v >>= 16 * (uint32_t)(at - from);
+    return v;
+}
 template <int GS, bool Z>
 __device__ __forceinline__ void l4_load(const qw_linear4_args &a, l4_step<GS, Z> &w, uint32_t col,
                                         uint32_t st, uint32_t g) {
@@ -61,13 +78,9 @@ __device__ __forceinline__ void l4_load(const qw_linear4_args &a, l4_step<GS, Z>
     uint32_t at = k0 + 32 * g;
     if (GS < 128) at = min(at, a.k - 32);
     w.q = *(const u32x4 *)(a.weight + ((size_t)col * a.k + at) / 2);
-    const size_t gi = (size_t)col * groups;
-#pragma unroll
-    for (int n = 0; n < 128 / GS; n++) {
-        const size_t e = gi + min(k0 / GS + n, groups - 1);
-        w.s[n] = a.scales[e];
-        w.z[n] = Z ? a.zeros[e] : 0x4100; /* 8 */
-    }
+    const uint64_t e = (uint64_t)col * groups + k0 / GS, all = (uint64_t)a.cols * groups;
+    w.s = l4_groups<GS>(a.scales, e, all);
+    w.z = Z ? l4_groups<GS>(a.zeros, e, all) : (l4_pack<GS>)0x4100410041004100ull; /* 8 */
 }
 
 /* ---- up to 16 rows that fit LDS ------------------------------------------- */
@@ -279,7 +292,7 @@ __device__ __forceinline__ void linear4_many(const qw_linear4_args &a) {
             }
 #pragma unroll
             for (int c = 0; c < CT; c++) {
-                const float s = bf2f(w[u][c].s[n]), z = -128.0f - bf2f(w[u][c].z[n]);
+                const float s = bf2f((u16)(w[u][c].s >> 16 * n)), z = -128.0f - bf2f((u16)(w[u][c].z >> 16 * n));
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
