@@ -852,7 +852,10 @@ __device__ __forceinline__ void pa_few(const qw_paged_args &a) {
 #pragma unroll
         for (int w = 0; w < PF_WAVES; w++) {
             const float m = row[w * SUMS + PA_D];
-            if (m == -INFINITY) continue; /* the wave saw no key of the row */
+            if (m == -INFINITY) { /* the wave saw no key of the row, or scores that are NaN */
+                l_all[rt] += row[w * SUMS + PA_D + 1];
+                continue;
+            }
             const float f = __builtin_amdgcn_exp2f(m - m_all[rt]);
             l_all[rt] = __builtin_fmaf(row[w * SUMS + PA_D + 1], f, l_all[rt]);
 #pragma unroll

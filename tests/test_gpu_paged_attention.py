@@ -169,6 +169,26 @@ def test_infinities_that_a_row_does_not_see(gpu, qd, past, new, heads, window):
     check(gpu, qd, rng, b, heads, window)
 
 
+@pytest.mark.parametrize("past, new, heads", [([30], [1], 4), ([2000], [1], 8), ([9000], [3], 8),
+                                             ([700], [40], 4), ([30, 500], [200, 90], 8)])
+def test_nan_in_q_and_in_stretches_of_k(gpu, qd, past, new, heads):
+    """NaN wherever the formula has it: a query of NaN, and keys of NaN over
+    whole tiles, where a wave or a piece sees nothing else."""
+    rng = np.random.default_rng(past[0])
+    b = ref.Batch(rng, past, new, 2, 16, fill=NAN)
+    for s in range(len(new)):
+        t, page, slot = b.slots(s)
+        at = slice(len(t) // 3, len(t) // 3 + 200)
+        b.k[page[at], slot[at], 1] = NAN
+    q = ref.normal(rng, b.rows, heads, 128, std=1.5)
+    q[b.rows // 2, 0] = NAN
+    out = np.full(q.shape, SENTINEL, np.uint16)
+    got = attend(gpu, qd, b, q, out)
+    ref.close(got, *ref.attention(b, q, out, SCALE))
+    assert np.isnan(ref.f64(got[b.rows // 2, 0])).all()
+    assert np.isnan(ref.f64(got[b.rows - 1, heads - 1])).all()
+
+
 @pytest.mark.parametrize("new", [1, 90])
 def test_scores_of_any_size(gpu, qd, new):
     """Rows whose keys give scores far apart, all very low or all equal: the
