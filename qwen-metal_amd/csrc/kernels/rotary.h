@@ -9,11 +9,14 @@
  * series of sine and cosine. Norm and rotation stay in fp32 and are rounded
  * once, at the store.
  *
- * Bound by HBM for many rows, by latency for few. A workgroup has one row and
- * 256 / (head_dim / 8) of its heads (or three times as many), a lane 16 bytes
- * of a head: the row's sines are made
- * once per workgroup and shared through LDS (made by every lane for itself
- * they cost 8 pairs for each 16 bytes, more than the bytes' time). */
+ * Bound by latency for few rows (one row into the cache 3.8 us, an empty launch
+ * 3.0: starts and lengths, the table's entry, the store), by HBM and close
+ * behind it by the vector unit for many (11900 rows of 32 + 8 heads, normed,
+ * into the cache 46.6 us, 4.1 TB/s; a large copy has 4.8). A workgroup has one
+ * row and 256 / (head_dim / 8) of its heads (or three times as many), a lane 16
+ * bytes of a head: the row's sines are made once per workgroup and shared
+ * through LDS (made by every lane for itself they cost 8 pairs for each 16
+ * bytes, more than the bytes' time). */
 #pragma once
 #include "common.h"
 #include "paged_cache.h"
@@ -43,9 +46,19 @@ __device__ __forceinline__ uint32_t rotary_sequence(const qw_cache_args &c, uint
     return n;
 }
 
+/* Not kept in L2, where the rows to come would have to push it out: 11900 rows
+ * of 32 + 8 heads into the cache 50.7 -> 46.6 us, 1000 rows of them beside it
+ * 6.2 -> 5.0. An attention that follows at once gains and loses nothing by it:
+ * both together 41.9 -> 41.3 us at 1000 rows, 250 -> 251.5 at 8400, 15.4 at
+ * one. */
+__device__ __forceinline__ void rotary_store(u16 *to, u32x4 v) {
+    __builtin_nontemporal_store(v, (u32x4 *)to);
+}
+
 /* H heads a lane: 1 for few rows, where the chain of loads to a row's page is
  * the time, 3 for many, where a row's chain, sines and norm weights serve 3
- * times the bytes. */
+ * times the bytes (the 11900 rows: 60 us with 1, 50 with 3, before the stores
+ * went past L2). */
 template <int D, int H>
 __device__ __forceinline__ void rotary_impl(const qw_rotary_args &a) {
     constexpr uint32_t LPH = D / 8, HPP = 256 / LPH; /* lanes per head, heads per pass */
@@ -165,11 +178,11 @@ __device__ __forceinline__ void rotary_impl(const qw_rotary_args &a) {
             for (int i = 0; i < 4; i++) own[n][i] = pack_bf(x[2 * i], x[2 * i + 1]);
         }
         if (is_q) {
-            *(u32x4 *)(a.q_out + (size_t)row * a.ldq_out + head * D + c8) = own[n];
+            rotary_store(a.q_out + (size_t)row * a.ldq_out + head * D + c8, own[n]);
         } else if (!a.cached) {
-            *(u32x4 *)(a.k_out + (size_t)row * a.ldk_out + kvh * D + c8) = own[n];
+            rotary_store(a.k_out + (size_t)row * a.ldk_out + kvh * D + c8, own[n]);
         } else if (at != ~0ull) {
-            *(u32x4 *)((is_k ? a.cache.k : a.cache.v) + at + kvh * D + c8) = own[n];
+            rotary_store((is_k ? a.cache.k : a.cache.v) + at + kvh * D + c8, own[n]);
         }
     }
 }
