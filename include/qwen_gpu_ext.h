@@ -306,8 +306,10 @@ int qw_gpu_copy_rows(h3_gpu *gpu, h3_gpu_tensor *dst, size_t dst_offset,
  * rows starts[s] .. starts[s + 1] - 1 of the batch, in order, the last of them
  * its last token; starts is ascending. Rows before starts[0] and from
  * starts[sequences] on belong to no sequence and are left as they are in every
- * output. page_size is a power of two from 8 to 4096. Sequences may share
- * pages that they only read; a page that a call writes belongs to one. */
+ * output. page_size is a power of two from 8 to 4096; a sequence's table has
+ * less than 2^31 tokens, the cache less than 2^32 and at most 1024 heads; at
+ * most 2^20 sequences. Sequences may share pages that they only read; a page
+ * that a call writes belongs to one. */
 typedef struct {
     h3_gpu_tensor *k, *v; /* bf16 [pages, page_size, kv_heads, head_dim] */
     const h3_gpu_tensor *table;   /* u32 [sequences, table_ld] */
@@ -332,7 +334,7 @@ enum { QW_ROTARY_INTERLEAVED = 0, QW_ROTARY_HALF = 1 };
  * q_out may be q (the same rows, in place) and k_out k; otherwise outputs and
  * inputs do not overlap. heads or kv_heads may be 0 (without a cache): then
  * nothing is done for q or k. head_dim 64, 128 or 256; rotary_dim even, up to
- * head_dim. Rows and norm weights are 16-byte aligned. */
+ * head_dim; less than 2^24 rows. Rows and norm weights are 16-byte aligned. */
 typedef struct {
     h3_gpu_tensor *q_out;
     size_t q_out_offset;
@@ -391,8 +393,12 @@ int qw_gpu_paged_attention_check(const qw_paged_attention_desc *desc, char *erro
  * input k of column c (the low half of byte k / 2 for even k), s = scales[c][k /
  * group] and z = zeros[c][k / group], 8 without zeros. Rows of in and out at
  * strides lda and ldc. fp32 sums, one rounding. group 32, 64 or 128; k a
- * multiple of it; cols of 8. Rows of in are 16-byte aligned, of out 8, the
- * weight 16, scales and zeros 4. The output overlaps no operand. */
+ * multiple of it, up to 2^20; cols of 8, below 2^30. Made for few rows: beyond
+ * 64 the weight is read once for every 64, and qw_gpu_dequant_int4_bf16 with
+ * qw_gpu_linear is the faster way. Rows of in are 16-byte aligned, of out 8, the
+ * weight 16, scales and zeros 4. The output overlaps no operand. An input that
+ * is infinite, or so large that 2^8 times a group's sum passes fp32, makes its
+ * row NaN or infinite. */
 typedef struct {
     h3_gpu_tensor *out;
     size_t out_offset;

@@ -99,6 +99,7 @@ def test_wrap(qd):
     (dict(q_out=lambda d: d["turns"]), "wrong dtype"),
     (dict(norm_q=lambda d: d["q"]), "norm"),
     (dict(q_offset=(1 << 64) - 8), "too small"),
+    (dict(rows=1 << 24), "2^24 rows"),
 ])
 def test_rotary_refusals(qd, memory, over, word):
     desc = rotary(qd, Maker(qd, memory), **over)
@@ -170,7 +171,7 @@ def test_attention_out_over_the_cache(qd, memory):
 @pytest.mark.parametrize("over, word", [
     (dict(), None), (dict(rows=0), None), (dict(group=32), None),
     (dict(group=16), "groups"), (dict(group=256), "groups"), (dict(k=96), "multiple"),
-    (dict(k=0), "multiple"), (dict(cols=12), "multiple of 8"), (dict(rows=6), "too small"),
+    (dict(k=0), "multiple"), (dict(cols=12), "multiple of 8"), (dict(cols=1 << 30), "below 2^30"), (dict(rows=6), "too small"),
     (dict(lda=120), "stride"), (dict(lda=132, rows=4), "aligned"), (dict(weight=lambda d: d["in_"]), "dtype"),
     (dict(scales=None), "missing"), (dict(out=lambda d: d["in_"]), "overlaps"),
     (dict(bias=lambda d: d["out"]), "overlaps"), (dict(ldc=20), "stride"),
