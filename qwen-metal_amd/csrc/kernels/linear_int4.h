@@ -92,12 +92,20 @@ __device__ __forceinline__ void l4_load(const qw_linear4_args &a, l4_step<GS, Z>
  * the weights (12288 -> 4096, one row: 21.0 us against 10.3 with groups of 128
  * and no zero points). Weights are loaded L4_AHEAD steps before their use,
  * over the end of a tile into the next. Rows past the last are computed as it,
- * and not stored; so are columns. */
+ * and not stored; so are columns.
+ *
+ * x decides how many workgroups a CU has: two where it takes 64 KB with the
+ * scales, one up to 144. Beyond, and for more rows, x goes through LDS in
+ * slabs, which costs its pieces' meeting (16 rows, 4096 -> 6144: 8.3 us here,
+ * 10.9 there; 4096 -> 24576 15.0 and 19.6; 4 rows, 12288 -> 4096 11.4 and
+ * 20.2). Bound by HBM with the way to the first weights: one row 4096 -> 24576
+ * 12.5 us (4.2 TB/s), 12288 -> 4096 with zero points 10.1, of which an empty
+ * launch is 3. */
 #define L4_AHEAD 4
-#define L4_LDS 65536 /* x, then two buffers of scales and zero points */
-template <int GS, bool Z>
+template <int GS, bool Z, int LDS>
 __device__ __forceinline__ void linear4_few(const qw_linear4_args &a) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds[L4_LDS];
+    /* x, then two buffers of scales and zero points */
+    __shared__ __attribute__((aligned(16))) unsigned char lds[LDS];
     __shared__ float part[L4_WAVES][256];
     const uint32_t tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -135,13 +143,29 @@ __device__ __forceinline__ void linear4_few(const qw_linear4_args &a) {
         }
     };
     copy_scales(tile, 0);
-    /* 16-byte chunk ch of a row at ch ^ (row % 16); zeros behind k */
-    for (uint32_t row = 0; row < a.rows; row++)
-        for (uint32_t ch = tid; ch < steps * 16; ch += 64 * L4_WAVES) {
-            u32x4 v = {0, 0, 0, 0};
-            if (8 * ch < a.k) v = *(const u32x4 *)(a.in + (size_t)row * a.lda + 8 * ch);
-            *(bf16x8 *)(lds + row * steps * 256 + ((ch ^ (row & 15)) << 4)) = l4_order(v);
-        }
+    /* 16-byte chunk ch of a row at ch ^ row; zeros behind k. Loads of some rows
+     * together: one after another they are a latency each (16 rows, 4096 ->
+     * 6144: 12.0 us against 8.3; 16 together 8.7). */
+    auto copy_x = [&](auto together) __attribute__((always_inline)) {
+        constexpr uint32_t XR = decltype(together)::value;
+        for (uint32_t ch = tid; ch < steps * 16; ch += 64 * L4_WAVES)
+            for (uint32_t row0 = 0; row0 < a.rows; row0 += XR) {
+                u32x4 v[XR];
+#pragma unroll
+                for (uint32_t n = 0; n < XR; n++)
+                    v[n] = *(const u32x4 *)(a.in + (size_t)min(row0 + n, a.rows - 1) * a.lda + min(8 * ch, a.k - 8));
+#pragma unroll
+                for (uint32_t n = 0; n < XR; n++) {
+                    const uint32_t row = row0 + n;
+                    if (8 * ch >= a.k) v[n] = u32x4{0, 0, 0, 0};
+                    if (row < a.rows) *(bf16x8 *)(lds + row * steps * 256 + ((ch ^ row) << 4)) = l4_order(v[n]);
+                }
+            }
+    };
+    if (LDS <= QW_L4_FEW && a.rows == 1)
+        copy_x(std::integral_constant<uint32_t, 1>());
+    else
+        copy_x(std::integral_constant<uint32_t, LDS <= QW_L4_FEW ? 4 : 8>());
     __syncthreads();
     floatx4 sum = {0, 0, 0, 0};
     const uint32_t xrow = min(i, a.rows - 1);
@@ -194,19 +218,20 @@ __device__ __forceinline__ void linear4_few(const qw_linear4_args &a) {
         __syncthreads();
     }
 }
-#define L4_FEW(gs)                                                                             \
-    QW_KERNEL void __launch_bounds__(64 * L4_WAVES, 4) qw_linear4_few_g##gs(qw_linear4_args a) { \
-        linear4_few<gs, false>(a);                                                             \
-    }                                                                                          \
-    QW_KERNEL void __launch_bounds__(64 * L4_WAVES, 4) qw_linear4_few_g##gs##z(qw_linear4_args a) { \
-        linear4_few<gs, true>(a);                                                              \
+#define L4_FEW(name, gs, lds, waves)                                                             \
+    QW_KERNEL void __launch_bounds__(64 * L4_WAVES, waves) qw_linear4_##name##_g##gs(qw_linear4_args a) { \
+        linear4_few<gs, false, lds>(a);                                                          \
+    }                                                                                            \
+    QW_KERNEL void __launch_bounds__(64 * L4_WAVES, waves) qw_linear4_##name##_g##gs##z(qw_linear4_args a) { \
+        linear4_few<gs, true, lds>(a);                                                           \
     }
-L4_FEW(32) L4_FEW(64) L4_FEW(128)
+L4_FEW(few, 32, QW_L4_FEW, 4) L4_FEW(few, 64, QW_L4_FEW, 4) L4_FEW(few, 128, QW_L4_FEW, 4)
+L4_FEW(wide, 32, QW_L4_WIDE, 2) L4_FEW(wide, 64, QW_L4_WIDE, 2) L4_FEW(wide, 128, QW_L4_WIDE, 2)
 
 /* ---- up to 64 rows ------------------------------------------------------- */
 
 /* x weighs as much as the weight: 16 columns a workgroup read it from L2
- * 1536 times for 24576 columns (98.8 us at 60 rows). A workgroup has 128
+ * 1536 times for 24576 columns (98.8 us at 60 rows, 32.5 here). A workgroup has 128
  * columns, 32 for each of 4 waves, and two such sets of waves on alternate
  * slabs of 128 inputs; x's slabs pass through LDS, in the order that l4_widen
  * gives weights, one pair of slabs ahead. Few columns are cut along K in

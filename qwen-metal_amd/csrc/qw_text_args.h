@@ -42,6 +42,10 @@ typedef struct {
     qw_cache_args cache;
 } qw_paged_args;
 
+/* Bytes of LDS for x and scales in the linears of few rows: two workgroups a
+ * CU, or one. */
+#define QW_L4_FEW 65536
+#define QW_L4_WIDE 147456
 typedef struct {
     uint16_t *out;
     const uint16_t *in;

@@ -59,6 +59,30 @@ def test_k_that_ends_inside_a_step(gpu, qd, group, k):
     ref.close(linear(gpu, qd, x, w, s, z, None, group), *ref.linear4(x, w, s, z, group))
 
 
+@pytest.mark.parametrize("rows, k, cols", [(1, 256, 16 * 1100 + 8), (3, 512, 16 * 600 + 8),
+                                           (16, 4096, 16 * 300 + 8), (5, 8320, 16 * 260 + 8)])
+@pytest.mark.parametrize("group, zeros", [(32, True), (64, False), (64, True), (128, True)])
+def test_more_columns_than_workgroups(gpu, qd, rows, k, cols, group, zeros):
+    """Several tiles of columns for some workgroups, of which a CU holds two (x
+    in 64 KB) or one."""
+    rng = np.random.default_rng(rows + group)
+    w, s, z = weight(rng, cols, k, group, zeros)
+    x, bias = ref.normal(rng, rows, k), ref.normal(rng, cols)
+    ref.close(linear(gpu, qd, x, w, s, z, bias, group), *ref.linear4(x, w, s, z, group, bias))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows, k", [(15, 4096), (16, 4224), (16, 4480), (4, 12288), (4, 16384), (8, 8192),
+                                     (9, 8192)])
+def test_x_about_what_lds_holds(gpu, qd, group, rows, k):
+    """x and the scales just inside and just outside of 144 KB."""
+    rng = np.random.default_rng(k + rows)
+    for zeros in (False, True):
+        w, s, z = weight(rng, 40, k, group, zeros)
+        x = ref.normal(rng, rows, k)
+        ref.close(linear(gpu, qd, x, w, s, z, None, group, lda=k + 8), *ref.linear4(x, w, s, z, group))
+
+
 @pytest.mark.parametrize("rows", [1, 20, 64])
 def test_every_weight_at_its_place(gpu, qd, rows):
     """Unit inputs pick single weights: (q - z) s exactly, one rounding."""
