@@ -892,9 +892,23 @@ __device__ __forceinline__ void pa_few(const qw_paged_args &a) {
         __syncthreads();
         if (arrived != used - 1) return;
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-        /* All pieces' m and l come to LDS with one latency; then `sets` of
-         * threads take every sets-th piece of a row's 8 columns each, and meet
-         * in LDS. */
+        /* `sets` of threads take every sets-th piece of a row's 8 columns each,
+         * and meet in LDS. The first four of them, which for a short context
+         * are all, are asked for here, with all pieces' m and l: one latency. */
+        const uint32_t sets = rows > 8 ? 1 : rows > 4 ? 2 : 4, per = 16 * PF_WAVES / 4 / sets; /* rows a pass */
+        const uint32_t set = tid / 16 / per;
+        floatx4 q[4][2];
+        auto load_o = [&](uint32_t row, uint32_t p0) __attribute__((always_inline)) {
+            const uint32_t at = (row * (PA_D + 4) + (tid & 15) * 8) * 4;
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    q[n][e] = __builtin_bit_cast(
+                        floatx4, __builtin_amdgcn_raw_buffer_load_b128(
+                                     pr, at + min(p0 + n * sets, used - 1) * SUMS * 4 + 16 * e, 0, 17));
+        };
+        load_o(tid / 16 % per, set);
         float *ml = (float *)lds; /* [row][piece][m | l], then a factor for m */
         for (uint32_t e = tid; e < used * rows; e += 64 * PF_WAVES) {
             const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(
@@ -921,24 +935,14 @@ __device__ __forceinline__ void pa_few(const qw_paged_args &a) {
         }
         __syncthreads();
         float *meet = total + BM;
-        const uint32_t sets = rows > 8 ? 1 : rows > 4 ? 2 : 4, per = 16 * PF_WAVES / 4 / sets; /* rows a pass */
-        const uint32_t set = tid / 16 / per;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             const uint32_t row = 16 * rt + tid / 16 % per;
 #pragma unroll
             for (int e = 0; e < 8; e++) acc[rt][e] = 0.0f;
             if (row < rows) {
-                const uint32_t at = (row * (PA_D + 4) + (tid & 15) * 8) * 4;
                 for (uint32_t p0 = set; p0 < used; p0 += 4 * sets) {
-                    floatx4 q[4][2];
-#pragma unroll
-                    for (int n = 0; n < 4; n++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            q[n][e] = __builtin_bit_cast(
-                                floatx4, __builtin_amdgcn_raw_buffer_load_b128(
-                                             pr, at + min(p0 + n * sets, used - 1) * SUMS * 4 + 16 * e, 0, 17));
+                    if (rt || p0 != set) load_o(row, p0);
 #pragma unroll
                     for (int n = 0; n < 4; n++) {
                         const uint32_t pc = p0 + n * sets;
