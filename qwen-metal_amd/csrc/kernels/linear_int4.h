@@ -231,22 +231,30 @@ L4_FEW(wide, 32, QW_L4_WIDE, 2) L4_FEW(wide, 64, QW_L4_WIDE, 2) L4_FEW(wide, 128
 /* ---- up to 64 rows ------------------------------------------------------- */
 
 /* x weighs as much as the weight: 16 columns a workgroup read it from L2
- * 1536 times for 24576 columns (98.8 us at 60 rows, 32.5 here). A workgroup has 128
- * columns, 32 for each of 4 waves, and two such sets of waves on alternate
- * slabs of 128 inputs; x's slabs pass through LDS, in the order that l4_widen
- * gives weights, one pair of slabs ahead. Few columns are cut along K in
- * a.pieces ranges that meet in memory (the last in adds them in order). NT:
- * tiles of 16 rows. */
-#define L4_COLS 128
-template <int NT, int GS, bool Z>
+ * 1536 times for 24576 columns (98.8 us at 60 rows, 30.7 here). A workgroup
+ * has 128 columns, 32 for each of 4 waves and two such sets of waves, or 96
+ * or 64 columns, 48 or 32 for each of two waves and four such sets. A set takes
+ * every 2nd or 4th slab of 128 inputs; x's slabs pass through LDS, in the order
+ * that l4_widen gives weights, one round of the sets ahead. The widest tile
+ * widens the fewest weights and reads the least of x, a narrower one fills the
+ * CUs where the widest leaves some idle: the host weighs them by measured
+ * times. Few columns are cut along K in a.pieces ranges that meet in memory
+ * (the last in adds them in order). NT: tiles of 16 rows.
+ *
+ * Bound by the issue of vector and matrix instructions: with 128 columns the
+ * same loop without any load from memory took 24 us of 32. The sums X, a third
+ * of the matrix instructions there, are a quarter with 48 columns a wave. */
+template <int NT, int COLS, int GS, bool Z>
 __device__ __forceinline__ void linear4_many(const qw_linear4_args &a) {
-    constexpr int ROWS = 16 * NT, CT = 2, SLAB = ROWS * 256; /* bytes */
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2][2 * SLAB];
+    constexpr int CW = COLS > 96 ? 4 : 2, SETS = L4_WAVES / CW, CT = COLS / CW / 16;
+    constexpr int ROWS = 16 * NT, SLAB = ROWS * 256 /* bytes */, N = CT * NT;
+    constexpr int XN = SETS * ROWS * 16 / 512; /* chunks of x of a thread */
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2][SETS * SLAB];
     __shared__ uint32_t arrived;
     const uint32_t tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), set = wave >> 2;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), set = wave / CW, part = wave % CW;
     const uint32_t piece = blockIdx.x % a.pieces, tile = blockIdx.x / a.pieces;
-    const uint32_t col0 = tile * L4_COLS + (wave & 3) * 32;
+    const uint32_t col0 = tile * COLS + part * (16 * CT);
     const uint32_t slabs = (a.k + 127) / 128;
     const uint32_t first = (uint64_t)slabs * piece / a.pieces;
     const uint32_t last = (uint64_t)slabs * (piece + 1) / a.pieces;
@@ -255,12 +263,12 @@ __device__ __forceinline__ void linear4_many(const qw_linear4_args &a) {
     uint32_t col[CT];
 #pragma unroll
     for (int c = 0; c < CT; c++) col[c] = min(col0 + 16 * c + i, a.cols - 1);
-    /* x: chunk n of a thread is 16 bytes of a row of one of the two slabs;
+    /* x: chunk n of a thread is 16 bytes of a row of one of the sets' slabs;
      * chunk ch of a row lies at ch ^ (row % 16) */
-    u32x4 xv[NT];
+    u32x4 xv[XN];
     auto load_x = [&](uint32_t slab) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
+        for (int n = 0; n < XN; n++) {
             const uint32_t c = n * 512 + tid, row = (c >> 4) % ROWS;
             const uint32_t k = (slab + c / (ROWS * 16)) * 128 + (c & 15) * 8;
             xv[n] = u32x4{0, 0, 0, 0};
@@ -269,7 +277,7 @@ __device__ __forceinline__ void linear4_many(const qw_linear4_args &a) {
     };
     auto store_x = [&](uint32_t buffer) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
+        for (int n = 0; n < XN; n++) {
             const uint32_t c = n * 512 + tid, row = (c >> 4) % ROWS;
             *(bf16x8 *)(lds[buffer] + c / (ROWS * 16) * SLAB + row * 256 +
                         (((c & 15) ^ (row & 15)) << 4)) = l4_order(xv[n]);
@@ -327,59 +335,58 @@ __device__ __forceinline__ void linear4_many(const qw_linear4_args &a) {
             }
         }
     };
-    /* slabs at, at + 1 (one a set) from buffer, weights of the two pairs after
-     * in flight */
+    /* slabs at, at + 1, ... (one a set) from buffer, weights of the two rounds
+     * after in flight */
     load_x(first);
     load_w(0, first + set);
-    load_w(1, first + 2 + set);
+    load_w(1, first + SETS + set);
     store_x(0);
-    load_x(first + 2);
+    load_x(first + SETS);
     __syncthreads();
     uint32_t buffer = 0;
-    for (uint32_t at = first; at < last; at += 4) {
+    for (uint32_t at = first; at < last; at += 2 * SETS) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const uint32_t s = at + 2 * u; /* the same for all waves */
+            const uint32_t s = at + SETS * u; /* the same for all waves */
             if (s >= last) break;
             if (s + set < last) step(u, buffer, (s + set) * 128);
-            load_w(u, s + 4 + set);
-            if (s + 2 < last) {
+            load_w(u, s + 2 * SETS + set);
+            if (s + SETS < last) {
                 store_x(buffer ^ 1);
-                load_x(s + 4);
+                load_x(s + 2 * SETS);
             }
             __syncthreads();
             buffer ^= 1;
         }
     }
-    /* the second set's sums to the first: 4 waves x 2 NT KB */
-    float *meet = (float *)lds + (wave & 3) * (CT * NT * 256);
-    static_assert(4 * CT * NT * 1024 <= sizeof(lds), "");
-    if (set) {
+    /* the sets' sums meet in LDS: set s adds up every SETS-th block of 16 x
+     * 16 from the s-th on, and has it from here on */
+    float *const meet = (float *)lds + part * (N * 256) + lane * 4;
+    static_assert(L4_WAVES * N * 1024 <= sizeof(lds), "");
 #pragma unroll
-        for (int c = 0; c < CT; c++)
-#pragma unroll
-            for (int t = 0; t < NT; t++) *(floatx4 *)(meet + (c * NT + t) * 256 + lane * 4) = sum[c][t];
-    }
+    for (int n = 0; n < N; n++) *(floatx4 *)(meet + (set * CW * N + n) * 256) = sum[n / NT][n % NT];
     __syncthreads();
-    if (!set) {
+    constexpr int OWN = (N + SETS - 1) / SETS;
+    floatx4 own[OWN];
 #pragma unroll
-        for (int c = 0; c < CT; c++)
+    for (int m = 0; m < OWN; m++) {
+        const uint32_t n = min(m * SETS + set, N - 1);
+        own[m] = floatx4{0, 0, 0, 0};
 #pragma unroll
-            for (int t = 0; t < NT; t++) sum[c][t] += *(const floatx4 *)(meet + (c * NT + t) * 256 + lane * 4);
+        for (int w = 0; w < SETS; w++) own[m] += *(const floatx4 *)(meet + (w * CW * N + n) * 256);
     }
     if (a.pieces > 1) {
-        constexpr uint32_t PB = 4 * CT * NT * 1024; /* bytes of a piece */
+        constexpr uint32_t PB = CW * N * 1024; /* bytes of a piece */
         const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
             (void *)((unsigned char *)a.part + (size_t)tile * a.pieces * PB), (short)0,
             (int)(a.pieces * PB), 0x00020000);
-        const uint32_t at = (wave & 3) * (CT * NT * 1024) + lane * 16;
-        if (!set) {
+        const uint32_t at = part * (N * 1024) + set * 1024 + lane * 16;
 #pragma unroll
-            for (int n = 0; n < CT * NT; n++)
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum[n / NT][n % NT]), pr,
-                                                       piece * PB + at + n * 1024, 0, 17);
-            __builtin_amdgcn_s_waitcnt(0x0F70); /* vmcnt(0): the piece's stores are done */
-        }
+        for (int m = 0; m < OWN; m++)
+            if (m * SETS + set < N)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, own[m]), pr,
+                                                       piece * PB + at + m * SETS * 1024, 0, 17);
+        __builtin_amdgcn_s_waitcnt(0x0F70); /* vmcnt(0): the piece's stores are done */
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
         __syncthreads();
         if (tid == 0)
@@ -387,42 +394,42 @@ __device__ __forceinline__ void linear4_many(const qw_linear4_args &a) {
         __syncthreads();
         if (arrived != a.pieces - 1) return;
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-        if (!set) {
 #pragma unroll
-            for (int n = 0; n < CT * NT; n++) sum[n / NT][n % NT] = floatx4{0, 0, 0, 0};
-            for (uint32_t pc = 0; pc < a.pieces; pc++)
+        for (int m = 0; m < OWN; m++) own[m] = floatx4{0, 0, 0, 0};
+        for (uint32_t pc = 0; pc < a.pieces; pc++)
 #pragma unroll
-                for (int n = 0; n < CT * NT; n++)
-                    sum[n / NT][n % NT] += __builtin_bit_cast(
-                        floatx4, __builtin_amdgcn_raw_buffer_load_b128(pr, pc * PB + at + n * 1024, 0, 17));
-        }
+            for (int m = 0; m < OWN; m++)
+                own[m] += __builtin_bit_cast(
+                    floatx4, __builtin_amdgcn_raw_buffer_load_b128(
+                                 pr, pc * PB + at + (min(m * SETS + set, N - 1) - set) * 1024, 0, 17));
         if (tid == 0)
             __hip_atomic_store(a.flag + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    if (set) return;
 #pragma unroll
-    for (int c = 0; c < CT; c++) {
-        if (col0 + 16 * c + i >= a.cols) continue;
-        const float b = a.bias ? bf2f(a.bias[col[c]]) : 0.0f;
+    for (int m = 0; m < OWN; m++) {
+        const uint32_t n = m * SETS + set, to = col0 + 16 * (n / NT) + i;
+        if (n >= N || to >= a.cols) continue;
+        const float b = a.bias ? bf2f(a.bias[to]) : 0.0f;
 #pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const uint32_t row = 16 * t + 4 * g + r;
-                if (row < a.rows) a.out[(size_t)row * a.ldc + col[c]] = f2bf(sum[c][t][r] + b);
-            }
+        for (int r = 0; r < 4; r++) {
+            const uint32_t row = 16 * (n % NT) + 4 * g + r;
+            if (row < a.rows) a.out[(size_t)row * a.ldc + to] = f2bf(own[m][r] + b);
+        }
     }
 }
-#define L4_MANY(nt, gs)                                                                        \
-    QW_KERNEL void __launch_bounds__(512, 2) qw_linear4_r##nt##_g##gs(qw_linear4_args a) {     \
-        linear4_many<nt, gs, false>(a);                                                        \
-    }                                                                                          \
-    QW_KERNEL void __launch_bounds__(512, 2) qw_linear4_r##nt##_g##gs##z(qw_linear4_args a) {  \
-        linear4_many<nt, gs, true>(a);                                                         \
+/* One workgroup a CU is what the host plans, so two waves a SIMD: with a third
+ * in mind the compiler asks for x later (60 rows, 4096 -> 32768: 39.0 us
+ * against 36.4). */
+#define L4_MANY(nt, cols, gs)                                                                           \
+    QW_KERNEL void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) qw_linear4_r##nt##_c##cols##_g##gs(qw_linear4_args a) {    \
+        linear4_many<nt, cols, gs, false>(a);                                                           \
+    }                                                                                                   \
+    QW_KERNEL void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) qw_linear4_r##nt##_c##cols##_g##gs##z(qw_linear4_args a) { \
+        linear4_many<nt, cols, gs, true>(a);                                                            \
     }
-L4_MANY(1, 32) L4_MANY(1, 64) L4_MANY(1, 128)
-L4_MANY(2, 32) L4_MANY(2, 64) L4_MANY(2, 128)
-L4_MANY(4, 32) L4_MANY(4, 64) L4_MANY(4, 128)
+#define L4_GROUPS(nt, cols) L4_MANY(nt, cols, 32) L4_MANY(nt, cols, 64) L4_MANY(nt, cols, 128)
+#define L4_TILES(cols) L4_GROUPS(1, cols) L4_GROUPS(2, cols) L4_GROUPS(4, cols)
+L4_TILES(64) L4_TILES(96) L4_TILES(128)
 
 /* One wave per 64 groups' worth of weights would waste lanes on short rows, so
  * a lane has a group of its own: two passes over its 32 to 128 weights (the

@@ -71,6 +71,20 @@ def test_more_columns_than_workgroups(gpu, qd, rows, k, cols, group, zeros):
     ref.close(linear(gpu, qd, x, w, s, z, bias, group), *ref.linear4(x, w, s, z, group, bias))
 
 
+@pytest.mark.parametrize("rows, k", [(16, 4608), (30, 384), (60, 640), (64, 256)])
+@pytest.mark.parametrize("cols", [16384 - 8, 16384 + 40, 24576 + 24, 33000])
+@pytest.mark.parametrize("group, zeros", [(32, True), (64, True), (128, False)])
+def test_a_round_of_workgroups(gpu, qd, rows, k, cols, group, zeros):
+    """Columns about what 256 workgroups of 64, 96 and 128 have; the last tiles
+    and columns drawn from the rest."""
+    rng = np.random.default_rng(rows + cols)
+    w, s, z = weight(rng, cols, k, group, zeros)
+    x, bias = ref.normal(rng, rows, k), ref.normal(rng, cols)
+    got = linear(gpu, qd, x, w, s, z, bias, group)
+    at = np.r_[0:200, np.sort(rng.choice(np.arange(200, cols - 200), 300, False)), cols - 200:cols]
+    ref.close(got[:, at], *ref.linear4(x, w[at], s[at], z[at] if zeros else None, group, bias[at]))
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("rows, k", [(15, 4096), (16, 4224), (16, 4480), (4, 12288), (4, 16384), (8, 8192),
                                      (9, 8192)])
