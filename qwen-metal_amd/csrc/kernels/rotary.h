@@ -11,7 +11,7 @@
  *
  * Bound by latency for few rows (one row into the cache 3.8 us, an empty launch
  * 3.0: starts and lengths, the table's entry, the store), by HBM and close
- * behind it by the vector unit for many (11900 rows of 32 + 8 heads, normed,
+ * behind it by the vector unit for many (7724 rows of 32 + 8 heads, normed,
  * into the cache 46.6 us, 4.1 TB/s; a large copy has 4.8). A workgroup has one
  * row and 256 / (head_dim / 8) of its heads (or three times as many), a lane 16
  * bytes of a head: the row's sines are made once per workgroup and shared
@@ -46,10 +46,10 @@ __device__ __forceinline__ uint32_t rotary_sequence(const qw_cache_args &c, uint
     return n;
 }
 
-/* Not kept in L2, where the rows to come would have to push it out: 11900 rows
+/* Not kept in L2, where the rows to come would have to push it out: 7724 rows
  * of 32 + 8 heads into the cache 50.7 -> 46.6 us, 1000 rows of them beside it
  * 6.2 -> 5.0. An attention that follows at once gains and loses nothing by it:
- * both together 41.9 -> 41.3 us at 1000 rows, 250 -> 251.5 at 8400, 15.4 at
+ * both together 41.9 -> 41.3 us at 1000 rows, 250 -> 251.5 at 7724, 15.4 at
  * one. */
 __device__ __forceinline__ void rotary_store(u16 *to, u32x4 v) {
     __builtin_nontemporal_store(v, (u32x4 *)to);
@@ -57,7 +57,7 @@ __device__ __forceinline__ void rotary_store(u16 *to, u32x4 v) {
 
 /* H heads a lane: 1 for few rows, where the chain of loads to a row's page is
  * the time, 3 for many, where a row's chain, sines and norm weights serve 3
- * times the bytes (the 11900 rows: 60 us with 1, 50 with 3, before the stores
+ * times the bytes (the 7724 rows: 60 us with 1, 50 with 3, before the stores
  * went past L2). */
 template <int D, int H>
 __device__ __forceinline__ void rotary_impl(const qw_rotary_args &a) {
