@@ -70,7 +70,7 @@ static const char *k_names[K_COUNT] = {
 enum { QW_INT8_AUTO = 0, QW_INT8_WIDEN = 1, QW_INT8_W8 = 2 };
 
 #define QW_SPAN_MAX 4096
-enum { T_COUNT = 79 }; /* kernels of the text operators (h3_gpu_text.inc) */
+enum { T_COUNT = 80 }; /* kernels of the text operators (h3_gpu_text.inc) */
 
 struct h3_gpu {
     int device;

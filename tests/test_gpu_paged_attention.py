@@ -123,7 +123,8 @@ def test_long_contexts_in_pieces(gpu, qd, heads, kv, past, page, window):
         assert np.array_equal(attend(gpu, qd, b, q, out, window), got)
 
 
-@pytest.mark.parametrize("past, new", [([3000], [40]), ([1500, 600], [70, 90])])
+@pytest.mark.parametrize("past, new", [([3000], [40]), ([1500, 600], [70, 90]), ([16000], [20]),
+                                       ([50000, 3000], [9, 30])])
 def test_chunks_in_pieces(gpu, qd, past, new):
     rng = np.random.default_rng(past[0])
     b = ref.Batch(rng, past, new, 2, 64, fill=NAN)
@@ -150,7 +151,8 @@ def test_a_piece_of_many_page_ids(gpu, qd):
 
 
 @pytest.mark.parametrize("past, new, heads", [([70], [1], 4), ([40], [3], 8), ([0], [100], 4),
-                                             ([90, 0], [40, 64], 8), ([2000], [40], 4)])
+                                             ([90, 0], [40, 64], 8), ([2000], [40], 4),
+                                             ([16000], [20], 8)])
 @pytest.mark.parametrize("window", [0, 30])
 def test_infinities_that_a_row_does_not_see(gpu, qd, past, new, heads, window):
     """NaN and infinities in K and V of late and early tokens: rows that see
@@ -170,7 +172,8 @@ def test_infinities_that_a_row_does_not_see(gpu, qd, past, new, heads, window):
 
 
 @pytest.mark.parametrize("past, new, heads", [([30], [1], 4), ([2000], [1], 8), ([9000], [3], 8),
-                                             ([700], [40], 4), ([30, 500], [200, 90], 8)])
+                                             ([700], [40], 4), ([30, 500], [200, 90], 8),
+                                             ([16000], [20], 8)])
 def test_nan_in_q_and_in_stretches_of_k(gpu, qd, past, new, heads):
     """NaN wherever the formula has it: a query of NaN, and keys of NaN over
     whole tiles, where a wave or a piece sees nothing else."""
