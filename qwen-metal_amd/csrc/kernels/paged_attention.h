@@ -11,8 +11,8 @@
  * v_mfma_f32_32x32x16_bf16, K and V straight into LDS, QK of the next tile
  * under the softmax), bound by the matrix cores and the softmax's vector work
  * beside them: 32 heads on 8, four prompts of 2324 to 4096 tokens 365 to 390 us
- * by board (0.84 to 0.89 PFLOP/s), 512 tokens at 7937 88 us, of which the
- * pieces' meeting is 8 to 10. Few rows (single tokens): 16 or 32 rows on
+ * by board (0.84 to 0.89 PFLOP/s), 512 tokens at 7937 in 3 pieces 88 us. Few
+ * rows (single tokens): 16 or 32 rows on
  * v_mfma_f32_16x16x32_bf16, every wave streaming key tiles of its own through
  * its own part of LDS without a barrier, bound by HBM: 64 users of 4100 to 8192
  * keys 309 us (5.2 TB/s), two of 131000 and 91773 171 us (5.3). One user of
